@@ -196,11 +196,104 @@ PH_API int phobos_kda(const PhTensor *Q, const PhTensor *K, const PhTensor *V, c
  * reference's own check computes it (main.rs:1179-1188).                                 */
 PH_API int phobos_saxpy(const PhTensor *x, const PhTensor *y, const PhTensor *out, float alpha, void *stream);
 
+/* ---- 4-bit weights ----------------------------------------------------------------- *
+ * No counterpart in the reference: the products of a model that answers from 4-bit weights.
+ * Y[M,N] = alpha * X[M,K] W[N,K]^T + beta * Y with W[n,k] = scale[n,k/group] *
+ * (code[n,k] - zero[n,k/group]), codes 0..15, group 32, 64 or 128, K a multiple of group.
+ * X is f16, Y f16 or f32 (f32 sums, rounded once); Y is not read when beta == 0.
+ * X: rows 16-byte aligned.  Y: any N, any row stride >= N.
+ * phobos_q4_pack lays weights out once, in the order the kernel reads them: codes [N,K] one
+ * per byte (the low four bits count), scales and zeros [N, K/group] f16 (zeros may be NULL:
+ * 8) -> `packed`, a rank-1 i8 tensor of phobos_q4_packed_bytes(N, K, group) bytes (0 for
+ * sizes that are not supported).                                                          */
+PH_API size_t phobos_q4_packed_bytes(int64_t N, int64_t K, int32_t group);
+PH_API int phobos_q4_pack(const PhTensor *codes, const PhTensor *scales, const PhTensor *zeros, int32_t group,
+                          const PhTensor *packed, void *stream);
+PH_API int phobos_gemv_q4(const PhTensor *X, const PhTensor *packed, const PhTensor *Y, float alpha, float beta,
+                          int32_t group, void *stream);
+
+/* ---- key/value cache in 4 bits ------------------------------------------------------- *
+ * No counterpart in the reference: flash_attention's keys and values kept between calls, in
+ * pages, as 4-bit codes with an f16 (scale, zero) pair per group of dims:
+ *   scale = f16((max - min) / 15), zero = min, code = rint((x - min) / scale)
+ *   value = zero + scale * code
+ * A group that holds a value that is not finite reads back as NaN.  All arrays are device
+ * memory of the caller:
+ *   pages   [layers][n_pages][phobos_kv4_page_bytes], 16-byte aligned; layers layer_pitch
+ *           bytes apart (a multiple of 16)
+ *   refs    [n_pages]  sequences that hold a page; 0 = free.  Start with zeros.
+ *   tables  [max_seqs][table_width]  the pages of a sequence, in order
+ *   lens    [max_seqs]  its tokens.  Start with zeros.
+ * One page id stands for that page in every layer.  Calls enqueue on `stream`; calls that
+ * change the same cache must be ordered by the caller.
+ *
+ * A batch names sequences by `slots` [n] and rows by `indptr` [n + 1] (ascending, from 0) or
+ * NULL for one row each: rows indptr[i] .. indptr[i+1] - 1 of the tensors are the LAST tokens
+ * of sequence slots[i], whose length already counts them (phobos_kv4_extend).  Rows behind
+ * indptr[n] are left as they are.  A slot or page id out of range is never followed: the
+ * tokens it stands for count as absent and phobos_device_status reports PH_ERR_INVALID.    */
+typedef struct PhKv4Cache {
+  void *pages;
+  int32_t *refs;
+  int32_t *tables;
+  int32_t *lens;
+  int64_t layer_pitch;
+  int32_t layers, n_pages;
+  int32_t page_tokens;        /* 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim;           /* 64 or 128 */
+  int32_t group;              /* 32, 64 or 128, at most head_dim */
+  int32_t max_seqs, table_width;
+} PhKv4Cache;
+PH_API size_t phobos_kv4_page_bytes(int32_t kv_heads, int32_t head_dim, int32_t group, int32_t page_tokens);
+
+/* K, V: [T, kv_heads * head_dim] f16, rows 16-byte aligned.  Writes the rows' tokens into `layer`; a row whose token
+ * is not in the cache (the sequence is shorter than its rows) is left out.  Two rows that name one token in one call
+ * (a slot listed twice) are not ordered.  A token in a page that several sequences share is written for all of them;
+ * phobos_kv4_extend copies such a page first. */
+PH_API int phobos_kv4_append(const PhKv4Cache *cache, int32_t layer, const PhTensor *K, const PhTensor *V,
+                             const int32_t *slots, const int32_t *indptr, int32_t n, void *stream);
+/* The inverse: the values of those tokens as f16 (at most +-65504); a row whose token is not in the cache reads as zero. */
+PH_API int phobos_kv4_read(const PhKv4Cache *cache, int32_t layer, const PhTensor *K, const PhTensor *V,
+                           const int32_t *slots, const int32_t *indptr, int32_t n, void *stream);
+
+/* O = softmax(scale * q K^T) V over the cache.  Q, O: [T, q_heads * head_dim] f16, q_heads a multiple of kv_heads
+ * (head h reads key/value head h / (q_heads / kv_heads)).  The row of position p sees tokens j <= p, and with
+ * window > 0 only j > p - window.  A row that sees nothing gets zeros.  lse, [T, q_heads] f32 or NULL: the natural
+ * logarithm of the sum of exp(scale * q k), -inf for a row that sees nothing.  The workspace (256-byte aligned,
+ * phobos_kv4_attention_workspace_bytes; its contents need not be kept) joins what several CTAs found of one sequence;
+ * calls that share one must not overlap on the GPU. */
+PH_API size_t phobos_kv4_attention_workspace_bytes(const PhKv4Cache *cache, int64_t T, int32_t n, int32_t q_heads);
+PH_API int phobos_kv4_attention(const PhKv4Cache *cache, int32_t layer, const PhTensor *Q, const PhTensor *O,
+                                const PhTensor *lse, float scale, int32_t window, const int32_t *slots,
+                                const int32_t *indptr, int32_t n, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bookkeeping.  Fresh pages are the lowest free ids, handed out in the order of the rows.  `workspace` (256-byte
+ * aligned, phobos_kv4_pages_workspace_bytes; contents need not be kept).  shortfall (device, one value): 0 when done;
+ * > 0 when that many pages are missing, -1 when the request is wrong (a slot out of range or listed twice, a negative
+ * count, more tokens than table_width pages hold, a destination that is not empty): then nothing has changed. */
+PH_API size_t phobos_kv4_pages_workspace_bytes(const PhKv4Cache *cache);
+/* Makes room for counts[i] more tokens of slots[i] and adds them to its length.  A last page that others share and
+ * that the new tokens would be written to is copied, in all layers, as if the rows were taken one after another. */
+PH_API int phobos_kv4_extend(const PhKv4Cache *cache, const int32_t *slots, const int32_t *counts, int32_t n,
+                             int32_t *shortfall, void *workspace, size_t workspace_bytes, void *stream);
+/* Makes the empty sequences dst[i] continue from src[i]: sharing its pages, or with deep != 0 with copies of them. */
+PH_API int phobos_kv4_fork(const PhKv4Cache *cache, const int32_t *src, const int32_t *dst, int32_t n, int32_t deep,
+                           int32_t *shortfall, void *workspace, size_t workspace_bytes, void *stream);
+/* Shortens slots[i] to keep[i] tokens (keep NULL: to none) and gives the pages behind them back.  Rows that would not
+ * shorten it, and slots out of range, are left out; of several rows for one slot the first counts. */
+PH_API int phobos_kv4_free(const PhKv4Cache *cache, const int32_t *slots, const int32_t *keep, int32_t n, void *stream);
+/* Moves the pages in use to ids 0 .. L - 1 in all layers and renames them in refs and tables; writes L to `live`
+ * (device, one value).  Pages of id >= L keep their bytes and are free. */
+PH_API int phobos_kv4_compact(const PhKv4Cache *cache, int32_t *live, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
 /* ---- launch by entry name -------------------------------------------------- *
  * The COMPUTE operand model: Op::Compute{kernel, args, scalars, grid, cta}
  * (phobos-cluster/src/isa.rs:38-44).  `entry` is the PTX entry name the
  * reference would look up (= kernel name, phobos-lang/src/codegen/kernel.rs:90-93):
- * "gemm", "matmul", "matmul_init", "flash_attention", "saxpy", "kda".  Tensors are in
+ * "gemm", "matmul", "matmul_init", "flash_attention", "saxpy", "kda", and this library's
+ * own "gemv_q4" (X, packed, Y, alpha, beta, i32 group).  Tensors are in
  * signature order; scalars carry their parameter position.  `grid` and `cta`
  * describe the reference's own device tiling and are validated for presence
  * only.  The GEMM regime follows from the element types unless `kind_hint`

@@ -72,6 +72,15 @@ int device_state(DeviceState** out) {
   return PH_OK;
 }
 
+int device_props(int* sm_count, uint32_t** status) {
+  DeviceState* ds;
+  const int rc = device_state(&ds);
+  if (rc) return rc;
+  *sm_count = ds->sm_count;
+  *status = ds->status;
+  return PH_OK;
+}
+
 // ---- tensor validation ------------------------------------------------------------
 struct View {
   char* base;  // ptr + offset, in bytes
@@ -112,7 +121,7 @@ static int view_of(const PhTensor* t, const char* name, View* v) {
   return PH_OK;
 }
 
-static int map_launch_rc(int rc, const char* what, const char* err) {
+int map_launch_rc(int rc, const char* what, const char* err) {
   if (rc == 0) return PH_OK;
   if (rc == -2) return fail(PH_ERR_UNSUPPORTED, "%s: %s", what, err);
   if (rc == -1) return fail(PH_ERR_INVALID, "%s: %s", what, err);
@@ -142,7 +151,7 @@ size_t gemm_staging_bytes(long long M, long long N, long long K) {
 }
 
 // SM count of the current device if one is usable, else that of a B200.
-static int sm_count_or_default() {
+int sm_count_or_default() {
   DeviceState* ds;
   if (device_state(&ds) == PH_OK) return ds->sm_count;
   clear_error();
@@ -200,6 +209,10 @@ int phobos_device_status(void* stream, uint32_t* status_out) {
   if (e != cudaSuccess) return fail(PH_ERR_DEVICE, "status read: %s", cudaGetErrorString(e));
   if (w != 0) cudaMemset(ds->status, 0, sizeof(w));
   if (status_out) *status_out = w;
+  // site codes from 0x80 up: a kernel left out an access that the caller's device-side indices asked for (kv4.cuh)
+  if ((w & 0xff) >= 0x80)
+    return fail(PH_ERR_INVALID, "a kernel met a%s out of range (block %u)",
+                (w & 0xff) == 0x81 ? " sequence slot" : " page table entry or a position", w >> 8);
   if (w != 0) return fail(PH_ERR_TIMEOUT, "a device-side wait gave up (site 0x%x, block %u)", w & 0xff, w >> 8);
   return PH_OK;
 }
@@ -529,6 +542,16 @@ int phobos_launch(const char* entry, const PhTensor* t, int32_t n_tensors, const
     float scale;
     if ((rc = scalar_f32(scalars, n_scalars, 5, &scale))) return rc;
     return phobos_kda(&t[0], &t[1], &t[2], &t[3], &t[4], scale, stream);
+  }
+  if (!strcmp(entry, "gemv_q4")) {
+    // gemv_q4(X, W, Y, alpha, beta, group): W the packed weights, a rank-1 i8 tensor; group an i32 scalar
+    if (n_tensors != 3) return fail(PH_ERR_INVALID, "gemv_q4 takes 3 tensors, got %d", n_tensors);
+    float alpha, beta;
+    if ((rc = scalar_f32(scalars, n_scalars, 3, &alpha)) || (rc = scalar_f32(scalars, n_scalars, 4, &beta))) return rc;
+    for (int32_t i = 0; i < n_scalars; i++)
+      if (scalars[i].pos == 5 && scalars[i].dtype == PH_I32)
+        return phobos_gemv_q4(&t[0], &t[1], &t[2], alpha, beta, static_cast<int32_t>(scalars[i].bits), stream);
+    return fail(PH_ERR_INVALID, "gemv_q4: missing i32 scalar `group` at parameter position 5");
   }
   if (!strcmp(entry, "saxpy")) {
     // saxpy(x, y, out, alpha): examples/saxpy_fp32.ph

@@ -88,4 +88,51 @@ int launch_saxpy(const float* x, const float* y, float* out, unsigned long long 
 int launch_f32_to_f16_2d(const float* in, long long ld_in, void* out, long long rows, long long cols,
                          cudaStream_t stream, const char** err);
 
+// gemv_q4.cu — products with 4-bit weights (block layout at the top of that file).
+size_t q4_packed_bytes(long long N, long long K, int group);
+int launch_q4_pack(const void* codes, long long ldc, const void* scales, long long lds, const void* zeros, long long ldz,
+                   void* out, int N, int K, int group, cudaStream_t stream, const char** err);
+int launch_gemv_q4(const void* X, long long ldx, const void* W, void* Y, long long ldy, int out_f32, int M, int N, int K,
+                   int group, float alpha, float beta, int sm_count, uint32_t* status, cudaStream_t stream, const char** err);
+
+// The 4-bit key/value cache (layout in kv4.cuh): one layer of it for the kernels that read or write tokens.
+struct Kv4View {
+  uint8_t* pages;       // this layer's pages
+  int* refs;
+  int* tables;          // [max_seqs][table_width]
+  int* lens;            // [max_seqs]
+  long long page_bytes, layer_pitch;
+  int layers, n_pages, page_shift, heads, D, G, max_seqs, table_width;
+};
+
+// kv4_cache.cu — quantise rows into the pages, read rows back.
+int launch_kv4_append(const Kv4View& c, const void* K, long long ldk, const void* V, long long ldv, int T, const int* slots,
+                      const int* ind, int n, uint32_t* status, cudaStream_t stream, const char** err);
+int launch_kv4_read(const Kv4View& c, void* K, long long ldk, void* V, long long ldv, int T, const int* slots, const int* ind,
+                    int n, uint32_t* status, cudaStream_t stream, const char** err);
+
+// kv4_attn.cu — attention over the cache.
+struct Kv4AttnArgs {
+  const void* Q;
+  void* O;
+  float* lse;           // may be null
+  long long ldq, ldo, ldl;
+  int T, n, q_heads, window;
+  const int* slots;
+  const int* ind;       // may be null: one row per sequence
+  float scale;
+};
+size_t kv4_attention_workspace(const Kv4View& c, int T, int n, int q_heads, int sm_count);
+int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, size_t workspace_bytes, int sm_count,
+                         uint32_t* status, cudaStream_t stream, const char** err);
+
+// kv4_pages.cu — the pages' bookkeeping and moves.
+size_t kv4_pages_workspace(const Kv4View& c);
+int launch_kv4_extend(const Kv4View& c, const int* slots, const int* counts, int n, int* shortfall, void* workspace,
+                      int sm_count, cudaStream_t stream, const char** err);
+int launch_kv4_fork(const Kv4View& c, const int* src, const int* dst, int n, int deep, int* shortfall, void* workspace,
+                    int sm_count, cudaStream_t stream, const char** err);
+int launch_kv4_free(const Kv4View& c, const int* slots, const int* keep, int n, cudaStream_t stream, const char** err);
+int launch_kv4_compact(const Kv4View& c, int* live, void* workspace, int sm_count, cudaStream_t stream, const char** err);
+
 }  // namespace ph

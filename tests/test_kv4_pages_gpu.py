@@ -1,0 +1,258 @@
+"""Pages of the 4-bit cache (extend, fork, free, compact) on a B200 against a model that takes the rows one after another.
+Everything is whole numbers and bytes: equality."""
+import copy
+import random
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+class Model:
+    """The bookkeeping in plain Python; `data[page]` names what a page holds."""
+
+    def __init__(self, n_pages, seqs, width, page):
+        self.refs, self.lens, self.page, self.width = [0] * n_pages, [0] * seqs, page, width
+        self.tables, self.data, self.stamp = [[] for _ in range(seqs)], list(range(n_pages)), n_pages
+
+    def need(self, n):
+        return -(-n // self.page)
+
+    def fresh(self):
+        for i, r in enumerate(self.refs):
+            if r == 0:
+                self.refs[i] = 1
+                return i
+        return None
+
+    def extend(self, slots, counts):
+        old = copy.deepcopy(self.__dict__)
+        want, seen, have = 0, set(), self.refs.count(0)
+        for s, c in zip(slots, counts):
+            if not 0 <= s < len(self.lens) or s in seen or c < 0 or self.lens[s] + c > self.width * self.page:
+                return -1
+            seen.add(s)
+        for s, c in zip(slots, counts):
+            n = self.lens[s]
+            if c and n % self.page and self.refs[self.tables[s][-1]] > 1:
+                want += 1
+                self.refs[self.tables[s][-1]] -= 1
+                p = self.fresh()
+                if p is not None:
+                    self.data[p] = self.data[self.tables[s][-1]]
+                    self.tables[s][-1] = p
+            for _ in range(self.need(n + c) - self.need(n)):
+                want += 1
+                p = self.fresh()
+                if p is not None:
+                    self.tables[s].append(p)
+            self.lens[s] = n + c
+        if want > have:
+            self.__dict__.update(old)
+            return want - have
+        return 0
+
+    def fork(self, src, dst, deep):
+        if any(not (0 <= a < len(self.lens) and 0 <= b < len(self.lens)) or self.lens[b] for a, b in zip(src, dst)) or len(set(dst)) < len(dst):
+            return -1
+        lens = list(self.lens)
+        if deep:
+            want, have = sum(self.need(lens[a]) for a in src), self.refs.count(0)
+            if want > have:
+                return want - have
+        for a, b in zip(src, dst):
+            if not lens[a]:
+                continue
+            if deep:
+                self.tables[b] = [self.fresh() for _ in self.tables[a]]
+                for p, q in zip(self.tables[a], self.tables[b]):
+                    self.data[q] = self.data[p]
+            else:
+                self.tables[b] = list(self.tables[a])
+                for p in self.tables[a]:
+                    self.refs[p] += 1
+            self.lens[b] = lens[a]
+        return 0
+
+    def free(self, slots, keep=None):
+        seen = set()
+        for i, s in enumerate(slots):
+            k = keep[i] if keep else 0
+            if not 0 <= s < len(self.lens) or s in seen:
+                continue
+            seen.add(s)
+            if not 0 <= k < self.lens[s]:
+                continue
+            for p in self.tables[s][self.need(k):]:
+                self.refs[p] -= 1
+            self.tables[s], self.lens[s] = self.tables[s][:self.need(k)], k
+
+    def compact(self):
+        live = sum(r > 0 for r in self.refs)
+        holes = [i for i in range(live) if self.refs[i] == 0]
+        movers = [i for i in range(live, len(self.refs)) if self.refs[i] > 0]
+        to = dict(zip(movers, holes))
+        for a, b in to.items():
+            self.refs[b], self.refs[a], self.data[b] = self.refs[a], 0, self.data[a]
+        self.tables = [[to.get(p, p) for p in t] for t in self.tables]
+        return live
+
+
+class Both:
+    def __init__(self, ph, dev, n_pages=64, seqs=12, width=20, page=16, layers=2, heads=1, D=64):
+        import torch
+        self.ph, self.dev, self.m = ph, dev, Model(n_pages, seqs, width, page)
+        self.cache = ph.Kv4Cache.create(layers, n_pages, heads, D, 64, page, seqs, width)
+        self.cache.pages.copy_(torch.randint(0, 256, self.cache.pages.shape, dtype=torch.uint8, device=dev))
+        self.start = self.cache.pages.clone()
+        self.ws = torch.full((ph.kv4_pages_workspace_bytes(self.cache),), 0xFF, dtype=torch.uint8, device=dev)
+        self.out = torch.full((1,), 55, dtype=torch.int32, device=dev)
+
+    def ints(self, v):
+        import torch
+        return torch.tensor(v, dtype=torch.int32, device=self.dev)
+
+    def extend(self, slots, counts):
+        self.ph.kv4_extend(self.cache, self.ints(slots), self.ints(counts), self.out, workspace=self.ws)
+        return self.same(self.m.extend(slots, counts))
+
+    def fork(self, src, dst, deep=False):
+        self.ph.kv4_fork(self.cache, self.ints(src), self.ints(dst), self.out, deep=deep, workspace=self.ws)
+        return self.same(self.m.fork(src, dst, deep))
+
+    def free(self, slots, keep=None):
+        self.ph.kv4_free(self.cache, self.ints(slots), None if keep is None else self.ints(keep))
+        self.m.free(slots, keep)
+        self.same(None)
+
+    def compact(self):
+        self.ph.kv4_compact(self.cache, self.out, workspace=self.ws)
+        return self.same(self.m.compact())
+
+    def same(self, said):
+        c, m = self.cache, self.m
+        if said is not None:
+            assert int(self.out) == said
+        assert self.ph.device_status() == 0
+        assert c.refs.tolist() == m.refs
+        assert c.lens.tolist() == m.lens
+        for s, t in enumerate(m.tables):
+            assert c.tables[s, :len(t)].tolist() == t, s
+        used = [p for p in range(len(m.refs)) if m.refs[p]]
+        if used:
+            import torch
+            assert torch.equal(c.pages[:, used], self.start[:, [m.data[p] for p in used]])
+        return said
+
+
+def test_extend_takes_the_lowest_free_pages(ph, dev):
+    b = Both(ph, dev)
+    assert b.extend([3, 0, 5], [1, 33, 16]) == 0
+    assert b.m.tables[3] == [0] and b.m.tables[0] == [1, 2, 3] and b.m.tables[5] == [4]
+    b.extend([0], [15])                 # fills the page
+    b.extend([0, 3], [1, 0])            # the next one; no tokens: nothing
+    b.free([5, 0], [3, 20])
+    assert b.extend([7, 5], [40, 30]) == 0
+    assert b.extend([], []) == 0
+
+
+def test_refused_requests_change_nothing(ph, dev):
+    b = Both(ph, dev, n_pages=10)
+    b.extend([0, 1], [50, 40])
+    assert b.extend([2, 3], [40, 1]) == 1          # 7 are taken, 4 asked for
+    assert b.extend([2, 2], [1, 1]) == -1
+    assert b.extend([2, 12], [1, 1]) == -1
+    assert b.extend([-1], [1]) == -1
+    assert b.extend([2], [-1]) == -1
+    assert b.extend([2], [20 * 16 + 1]) == -1
+    assert b.extend([2], [2 ** 31 - 1]) == -1
+    assert b.fork([0], [1]) == -1
+    assert b.fork([0, 0], [2, 2]) == -1
+    assert b.fork([0], [12]) == -1 and b.fork([-3], [4]) == -1
+    assert b.fork([0], [2], deep=True) == 1
+    assert b.extend([2, 3], [32, 16]) == 0
+
+
+def test_shared_pages_are_copied_when_they_grow(ph, dev):
+    b = Both(ph, dev)
+    b.extend([0, 1], [40, 32])
+    assert b.fork([0, 0, 1, 0], [4, 5, 6, 7]) == 0
+    assert b.extend([4, 6, 0], [3, 1, 20]) == 0    # 4 and 0 copy the half page; 6 starts a new one
+    assert b.extend([5, 7], [1, 1]) == 0           # 5 copies; 7 is left alone with the page and keeps it
+    b.free([0, 5])
+    assert b.fork([7, 3], [0, 5]) == 0             # 3 is empty: so is 5
+    assert b.extend([0, 7], [1, 0]) == 0
+
+
+def test_deep_fork_and_compact(ph, dev):
+    b = Both(ph, dev, layers=3, heads=8)
+    b.extend([0, 1, 2, 3], [100, 17, 64, 33])
+    assert b.fork([0, 3], [4, 5], deep=True) == 0
+    b.fork([2], [6])
+    b.free([0, 1], [40, 0])
+    live = b.compact()
+    assert live == 14 - 0 - 0 or live > 0
+    assert b.compact() == live                     # nothing left to move
+    b.extend([1, 6], [30, 5])
+    b.free(list(range(12)))
+    assert b.compact() == 0
+
+
+def test_free_odd_requests(ph, dev):
+    b = Both(ph, dev)
+    b.extend([0, 1, 2], [40, 40, 40])
+    b.free([0, 0, 1, 99, -1, 2], [17, 3, 40, 0, 0, -5])
+    b.free([0, 0, 0])
+    b.free([0, 1], [0, 16])
+    b.free([])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_histories(ph, dev, seed):
+    r = random.Random(seed)
+    b = Both(ph, dev, n_pages=r.choice([40, 90]), seqs=9, width=14, page=r.choice([16, 32]), layers=2)
+    for _ in range(60):
+        op = r.choice(["extend", "extend", "extend", "fork", "free", "free", "compact"])
+        slots = r.sample(range(9), r.randint(1, 6))
+        if op == "extend":
+            b.extend(slots, [r.choice([0, 1, 1, 5, 16, 50]) for _ in slots])
+        elif op == "fork":
+            empty = [s for s in range(9) if b.m.lens[s] == 0]
+            r.shuffle(empty)
+            dst = empty[:r.randint(0, 3)]
+            b.fork([r.randrange(9) for _ in dst], dst, deep=r.random() < 0.5)
+        elif op == "free":
+            b.free(slots[:3], None if r.random() < 0.3 else [r.randint(0, 60) for _ in slots[:3]])
+        else:
+            b.compact()
+
+
+def test_many_sequences_and_pages(ph, dev):
+    """More rows and pages than one pass of the planning block holds."""
+    r = random.Random(1)
+    n = 2500
+    b = Both(ph, dev, n_pages=9000, seqs=n, width=4, page=16, layers=1)
+    slots = list(range(n))
+    r.shuffle(slots)
+    assert b.extend(slots[:2000], [r.randint(0, 40) for _ in range(2000)]) == 0
+    dst = [s for s in range(n) if b.m.lens[s] == 0][:400]
+    assert b.fork([slots[i % 300] for i in range(len(dst))], dst) == 0
+    assert b.extend(slots[:1500], [r.randint(0, 3) for _ in range(1500)]) == 0
+    b.free(slots[100:1400])
+    b.compact()
+
+
+def test_refusals(ph, dev):
+    import torch
+    b = Both(ph, dev)
+    one = b.ints([1])
+    bad = [lambda: ph.kv4_extend(b.cache, one, one, b.out, workspace=b.ws[:100]), lambda: ph.kv4_extend(b.cache, one, one, b.out),
+           lambda: ph.kv4_extend(b.cache, one.long(), one, b.out, workspace=b.ws), lambda: ph.kv4_extend(b.cache, b.ints([1, 2]), one, b.out, workspace=b.ws),
+           lambda: ph.kv4_extend(b.cache, b.ints(list(range(13))), b.ints([0] * 13), b.out, workspace=b.ws),
+           lambda: ph.kv4_fork(b.cache, one, one, b.out, workspace=torch.empty(1 << 20, dtype=torch.uint8, device=dev)[8:]),
+           lambda: ph.kv4_compact(b.cache, torch.empty(0, dtype=torch.int32, device=dev), workspace=b.ws), lambda: ph.kv4_compact(b.cache, b.out),
+           lambda: ph.kv4_free(b.cache, b.ints([1, 2]), one)]
+    for f in bad:
+        with pytest.raises(ph.PhobosError):
+            f()
+    b.same(None)
