@@ -1,14 +1,28 @@
 // Attention over the 4-bit cache: o = softmax(scale q K^T) V, one pass over the tokens with the running maximum and sum.
 //
 // A group of G dims of a token is zero + step * code, so
-//   q . k = sum_G ( step (q . c) + zero (sum q) )         and       sum_j p_j v_j = sum_j (p_j step_j) c_j + sum_j p_j zero_j
-// The matrix unit sees the bare codes of K against q, and the bare codes of V against p * step; zeros go through f32.
+//   q . k = sum_G ( step (q . c) + zero (sum q) )
+//   sum_j p_j v_j = sum_j (p_j step_j) (c_j - 8) + sum_j p_j (zero_j + 8 step_j)
+// The matrix unit sees the bare codes of K against q, and the codes of V, centred, against p * step; the rest goes
+// through f32.  (Uncentred, the sums of c cancel against the zeros: with 131072 tokens that cost o a relative error of
+// 3.5e-3, from the cut of the matrix unit's running sum.)
 // S^T = K Q^T has the tokens as rows, so a K fragment is 16 tokens x 16 dims straight from the page, and P^T, whose
 // accumulator layout is transposed by one movmatrix per 8 x 8, is the B operand of O^T = V^T P^T.
 //
 // p * step is rounded to f16 (half a step of 2^-11, as flash_attention rounds its p).  step can be small, so it is
 // taken relative to a running power of two `e` (the largest exponent of a step so far, moved up like the maximum),
 // with p * step * 2^(14 - e) < 2^15: a weight keeps its eleven bits down to 2^-28 of the largest.
+//
+// Work: a problem is one sequence, one key/value head and 8 NT query rows (a row is one query token and one of the
+// heads that read the key/value head).  The units of 16 tokens of all problems form one line that is cut into equal
+// pieces, one per CTA; a CTA's warps cut each problem's part of the piece again.  On the line every problem stands
+// behind AT_START places that hold no units: what starting one costs, so that a piece of many short sequences is not
+// longer than one of a long sequence.  A problem whose units lie in one piece is finished there; one that was cut
+// leaves (m, l, o) of its parts in the workspace for a second, small kernel.
+// Each warp streams its units through a ring in shared memory with bulk copies (one per unit, 2176 bytes at D = G =
+// 128) that it issues itself: no barrier between warps while tokens last.
+#include <atomic>
+
 #include "kv4.cuh"
 #include "q4.cuh"
 
@@ -16,7 +30,10 @@ namespace ph {
 namespace {
 
 constexpr int AT_WARPS = 4;
+constexpr int AT_START = 16;             // places for starting a problem
+constexpr int AT_PIECE = AT_START + 16;  // a piece is at least that: a tile of four units for each warp
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+enum : uint32_t { SITE_KV4_RING = 0x41 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -26,300 +43,650 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2^n for -126 <= n <= 127
 __device__ __forceinline__ float pow2i(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
 
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* at) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    w[0] = v.x; w[1] = v.y;
+  }
+}
+
 struct AttnParams {
   Kv4View c;
   Kv4AttnArgs a;
-  int rep;
+  int rep, pieces;
+  struct Cut* cuts;  // per CTA: the problem that its piece ends inside of
+  float* part;  // per CTA two parts: of the problem its piece begins inside of, and of the one it ends inside of
   uint32_t* status;
 };
 
-// Running state of eight query rows in one warp: lane 4g + t keeps rows 2t and 2t + 1.  Sums of p and of p * zero are
-// the lane's own tokens' only, until the end.
-template <int D, int NG>
+// What the joining kernel has to know of a problem that starts in one piece and goes on behind it.
+struct Cut {
+  int parts;          // 0: none, or its units lie in one piece
+  int first;          // index of its first part in the workspace; the following ones are those that continue it in the
+  int next;           // pieces after it: next, next + 2, ...
+  int row_begin, n_rows, head, tile, unused;
+};
+
+// One row tile of one sequence and key/value head, and where its units lie on the line.
+struct Problem {
+  Kv4Rows rows;
+  int head, tile;
+  int u_begin, units;      // tokens [16 u_begin, 16 (u_begin + units))
+};
+
+// Units of every problem of sequence b, and their first; at least one, so that rows without a token are answered too.
+__device__ __forceinline__ int seq_units(const AttnParams& p, const Kv4Rows& r, int* begin) {
+  const int n = r.end - r.begin;
+  *begin = p.a.window > 0 ? max(r.length - n + 1 - p.a.window, 0) / KV4_UNIT : 0;
+  return max((r.length + KV4_UNIT - 1) / KV4_UNIT - *begin, 1);
+}
+template <int ROWS>
+__device__ __forceinline__ int seq_problems(const AttnParams& p, const Kv4Rows& r) {
+  return p.c.heads * (((r.end - r.begin) * p.rep + ROWS - 1) / ROWS);
+}
+
+// Length of the line.  A whole warp calls.
+template <int ROWS>
+__device__ long long line_length(const AttnParams& p) {
+  long long sum = 0;
+  for (int b = threadIdx.x & 31; b < p.a.n; b += 32) {
+    const Kv4Rows r = kv4_rows(p.c, p.a.slots, p.a.ind, b, p.a.T, p.status);
+    int begin;
+    sum += static_cast<long long>(seq_units(p, r, &begin) + AT_START) * seq_problems<ROWS>(p, r);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return sum;
+}
+
+// Walks the sequences, 32 at a time, from `*b` (which stands at `*line`) to the one that holds place `at`.  A whole warp
+// calls; false behind the last.
+template <int ROWS>
+__device__ bool find_sequence(const AttnParams& p, long long at, int* b, long long* line) {
+  const int lane = threadIdx.x & 31;
+  long long done = *line;
+  for (int i0 = *b; i0 < p.a.n; i0 += 32) {
+    long long places = 0;
+    if (i0 + lane < p.a.n) {
+      const Kv4Rows r = kv4_rows(p.c, p.a.slots, p.a.ind, i0 + lane, p.a.T, p.status);
+      int begin;
+      places = static_cast<long long>(seq_units(p, r, &begin) + AT_START) * seq_problems<ROWS>(p, r);
+    }
+    long long sum = places;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, done + sum > at);
+    if (past) {
+      const int k = __ffs(past) - 1;
+      *b = i0 + k;
+      *line = done + __shfl_sync(0xffffffffu, sum - places, k);
+      return true;
+    }
+    done += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
+// Running state of 8 NT query rows in one warp: lane 4g + t keeps rows 8k + 2t and 8k + 2t + 1.  Sums of p and of
+// p * zero are the lane's own tokens' only, until the end.
+template <int D, int NG, int NT>
 struct RowState {
-  float m[2], l[2], z[2][NG];
-  float o[D / 16][4];  // dims 32p + 4g + {0, 2} (even i: low nibbles), + {1, 3} (odd i) of rows 2t, 2t + 1
+  float m[2 * NT], l[2 * NT], z[2 * NT][NG];
+  float o[NT][D / 16][4];  // dims 32p + 4g + {0, 2} (even i: low nibbles), + {1, 3} (odd i) of rows 2t, 2t + 1
   int e;
 };
-
-template <int D, int NG>
+template <int D, int NG, int NT>
 struct Queries {
-  uint32_t b[D / 16][2];  // B operand: row g, the dims of matrix step i
-  float sum[2][NG];       // sums of q over a group, rows 2t and 2t + 1
+  uint32_t b[NT][D / 16][2];  // B operand: row g, the dims of matrix step i
+  float sum[2 * NT][NG];      // sums of q over a group
+  int lo[2 * NT], hi[2 * NT]; // the tokens that a row sees
 };
 
-template <int D, int NG>
-__device__ __forceinline__ void kv4_tile(const uint8_t* unit, int tok0, int lo0, int hi0, int lo1, int hi1, float cs,
-                                         const Queries<D, NG>& q, RowState<D, NG>& s) {
-  constexpr int J = D / 32, W = D / 8;
+template <int D, int NG, int NT, int UN, bool MASKED>
+__device__ __forceinline__ void kv4_tile(const uint8_t* stage, int tok0, uint32_t present, float cs, const Queries<D, NG, NT>& q,
+                                         RowState<D, NG, NT>& s) {
+  constexpr int J = D / 32, W = D / 8, UNIT = kv4_unit_bytes(D, D / NG);
   const int lane = threadIdx.x & 31, g = lane >> 2;
-  const uint32_t* kw0 = reinterpret_cast<const uint32_t*>(unit + lane * W);
-  const uint32_t* kw1 = reinterpret_cast<const uint32_t*>(unit + 4 * D + lane * W);
-  const uint32_t* vw0 = reinterpret_cast<const uint32_t*>(unit + 8 * D + lane * W);
-  const uint32_t* vw1 = reinterpret_cast<const uint32_t*>(unit + 12 * D + lane * W);
-  const __half2* kpar = reinterpret_cast<const __half2*>(unit + 16 * D);
-  const __half2* vpar = reinterpret_cast<const __half2*>(unit + 16 * D + 64 * NG);
   // ---- S^T -------------------------------------------------------------------------------------------------------
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // tokens g (0, 1) and g + 8 (2, 3), rows 2t and 2t + 1
+  float x[UN][NT][4];  // tokens g (0, 1) and g + 8 (2, 3), rows 2t and 2t + 1
 #pragma unroll
-  for (int grp = 0; grp < NG; grp++) {
-    float lo[4] = {}, hi[4] = {};
+  for (int u = 0; u < UN; u++) {
+    const uint8_t* unit = stage + u * UNIT;
+    uint32_t kw0[J], kw1[J];
+    load_words<J>(kw0, unit + lane * W);
+    load_words<J>(kw1, unit + 4 * D + lane * W);
+    const __half2* kpar = reinterpret_cast<const __half2*>(unit + 16 * D);
 #pragma unroll
-    for (int j = grp * J / NG; j < (grp + 1) * J / NG; j++) {
-      const uint32_t a = kw0[j], b = kw1[j];
-      mma_16816(lo, a & Q4_LO, b & Q4_LO, (a >> 8) & Q4_LO, (b >> 8) & Q4_LO, q.b[2 * j][0], q.b[2 * j][1]);
-      mma_16816(hi, a & Q4_HI, b & Q4_HI, (a >> 8) & Q4_HI, (b >> 8) & Q4_HI, q.b[2 * j + 1][0], q.b[2 * j + 1][1]);
-    }
-    const float2 pa = __half22float2(kpar[g * NG + grp]), pb = __half22float2(kpar[(g + 8) * NG + grp]);
+    for (int k = 0; k < NT; k++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 p = i < 2 ? pa : pb;
-      const float dot = fmaf(hi[i], 1.0f / 16.0f, lo[i]) * Q4_LO_UNIT;
-      x[i] = fmaf(p.x, dot, fmaf(p.y, q.sum[i & 1][grp], x[i]));
+      for (int i = 0; i < 4; i++) x[u][k][i] = 0.0f;
+#pragma unroll
+    for (int grp = 0; grp < NG; grp++) {
+      float lo[NT][4] = {}, hi[NT][4] = {};
+#pragma unroll
+      for (int j = grp * J / NG; j < (grp + 1) * J / NG; j++) {
+        const uint32_t a = kw0[j], b = kw1[j], a2 = a >> 8, b2 = b >> 8;
+#pragma unroll
+        for (int k = 0; k < NT; k++) {
+          mma_16816(lo[k], a & Q4_LO, b & Q4_LO, a2 & Q4_LO, b2 & Q4_LO, q.b[k][2 * j][0], q.b[k][2 * j][1]);
+          mma_16816(hi[k], a & Q4_HI, b & Q4_HI, a2 & Q4_HI, b2 & Q4_HI, q.b[k][2 * j + 1][0], q.b[k][2 * j + 1][1]);
+        }
+      }
+      const float2 pa = __half22float2(kpar[g * NG + grp]), pb = __half22float2(kpar[(g + 8) * NG + grp]);
+      const float sa = pa.x * cs, sb = pb.x * cs;
+#pragma unroll
+      for (int k = 0; k < NT; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          x[u][k][i] = fmaf(i < 2 ? sa : sb, fmaf(hi[k][i], 1.0f / 16.0f, lo[k][i]),
+                            fmaf(i < 2 ? pa.y : pb.y, q.sum[2 * k + (i & 1)][grp], x[u][k][i]));
     }
   }
-  bool see[4];
+  auto sees = [&](int u, int k, int i) {
+    if (!MASKED) return true;
+    const int tok = tok0 + u * KV4_UNIT + g + (i >> 1) * 8, r = 2 * k + (i & 1);
+    return tok >= q.lo[r] && tok < q.hi[r] && ((present >> u) & 1u) != 0;
+  };
+  // ---- running maximum and weights -------------------------------------------------------------------------------------
+  float f[2 * NT];
+  bool moved = false;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int tok = tok0 + g + (i >> 1) * 8;
-    see[i] = (i & 1) ? (tok >= lo1 && tok < hi1) : (tok >= lo0 && tok < hi0);
-    x[i] = see[i] ? x[i] * cs : -INFINITY;
-  }
-  // ---- running maximum -----------------------------------------------------------------------------------------------
+  for (int r = 0; r < 2 * NT; r++) {
+    float m = s.m[r];
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    float m = fmaxf(x[r], x[2 + r]);
+    for (int u = 0; u < UN; u++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float& v = x[u][r >> 1][2 * h + (r & 1)];
+        if (MASKED && !sees(u, r >> 1, 2 * h + (r & 1))) v = -INFINITY;
+        m = fmaxf(m, v);
+      }
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-    m = fmaxf(m, s.m[r]);
-    const float f = s.m[r] == m ? 1.0f : exp2_approx(s.m[r] - m);  // (also where both are -inf)
+    f[r] = s.m[r] == m ? 1.0f : exp2_approx(s.m[r] - m);  // (1 also where both are -inf)
+    moved = moved || s.m[r] != m;
     s.m[r] = m;
-    s.l[r] *= f;
-#pragma unroll
-    for (int grp = 0; grp < NG; grp++) s.z[r][grp] *= f;
-#pragma unroll
-    for (int i = 0; i < D / 16; i++) {
-      s.o[i][r] *= f;
-      s.o[i][2 + r] *= f;
-    }
-  }
-  float p[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    p[i] = see[i] ? exp2_approx(x[i] - s.m[i & 1]) : 0.0f;
-    s.l[i & 1] += p[i];
   }
   // ---- the power of two that p * step is taken relative to ---------------------------------------------------------------
-  float step[2][NG];
-  uint32_t top = 0;
+  uint32_t top = 0, vpar[UN][2][NG];
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const bool any = see[2 * h] || see[2 * h + 1];
+  for (int u = 0; u < UN; u++) {
+    const uint32_t* at = reinterpret_cast<const uint32_t*>(stage + u * UNIT + 16 * D + 64 * NG);
 #pragma unroll
-    for (int grp = 0; grp < NG; grp++) {
-      const float2 v = __half22float2(vpar[(g + 8 * h) * NG + grp]);
-      step[h][grp] = v.x;
-      if (any && v.x <= 65504.0f) top = max(top, __float_as_uint(v.x) >> 23);
+    for (int h = 0; h < 2; h++) {
+      bool any = !MASKED;
 #pragma unroll
-      for (int r = 0; r < 2; r++)
-        if (see[2 * h + r]) s.z[r][grp] = fmaf(p[2 * h + r], v.y, s.z[r][grp]);
+      for (int k = 0; k < NT; k++) any = any || sees(u, k, 2 * h) || sees(u, k, 2 * h + 1);
+#pragma unroll
+      for (int grp = 0; grp < NG; grp++) {
+        vpar[u][h][grp] = at[(g + 8 * h) * NG + grp];
+        const uint32_t step = vpar[u][h][grp] & 0x7fffu;
+        if (any && step < 0x7c00u) top = max(top, step);
+      }
     }
   }
-  const int e = max(s.e, static_cast<int>(__reduce_max_sync(0xffffffffu, top & 255u)) - 127);
-  if (e != s.e) {
-    const float f = pow2i(max(s.e - e, -126));
+  // exponent of the largest finite step: a half's 2^(field - 15), and -14 for the subnormals
+  const int e = max(s.e, max(static_cast<int>(__reduce_max_sync(0xffffffffu, top) >> 10), 1) - 15);
+  if (__any_sync(0xffffffffu, moved) || e != s.e) {
+    const float down = pow2i(s.e - e);
 #pragma unroll
-    for (int i = 0; i < D / 16; i++)
+    for (int r = 0; r < 2 * NT; r++) {
+      s.l[r] *= f[r];
 #pragma unroll
-      for (int k = 0; k < 4; k++) s.o[i][k] *= f;
+      for (int grp = 0; grp < NG; grp++) s.z[r][grp] *= f[r];
+      const float fd = f[r] * down;
+#pragma unroll
+      for (int i = 0; i < D / 16; i++) {
+        s.o[r >> 1][i][r & 1] *= fd;
+        s.o[r >> 1][i][2 + (r & 1)] *= fd;
+      }
+    }
     s.e = e;
   }
   const float up = pow2i(14 - e);
-  // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------------------
 #pragma unroll
-  for (int grp = 0; grp < NG; grp++) {
-    float w[4];
+  for (int u = 0; u < UN; u++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = see[i] ? p[i] * (step[i >> 1][grp] * up) : 0.0f;
-    const uint32_t b0 = transpose_8x8(pack_half2(w[0], w[1])), b1 = transpose_8x8(pack_half2(w[2], w[3]));
+    for (int k = 0; k < NT; k++)
 #pragma unroll
-    for (int i = grp * J / NG; i < (grp + 1) * J / NG; i++) {
-      const uint32_t a = vw0[i], b = vw1[i];
-      mma_16816(s.o[2 * i], a & Q4_LO, (a >> 8) & Q4_LO, b & Q4_LO, (b >> 8) & Q4_LO, b0, b1);
-      mma_16816(s.o[2 * i + 1], a & Q4_HI, (a >> 8) & Q4_HI, b & Q4_HI, (b >> 8) & Q4_HI, b0, b1);
-    }
-  }
-}
-
-// One CTA: eight query rows (a row is one query token and one head of a key/value head's heads) of one sequence and one
-// key/value head; its warps share out the sequence's units and join at the end.
-template <int D, int NG>
-__global__ void __launch_bounds__(AT_WARPS * 32) kv4_attn_kernel(AttnParams p) {
-  constexpr int J = D / 32, G = D / NG, UNIT = kv4_unit_bytes(D, G);
-  __shared__ float so[AT_WARPS][8][D + 4];
-  __shared__ float sm[AT_WARPS][8], sl[AT_WARPS][8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int head = blockIdx.y;
-  // ---- which sequence and rows --------------------------------------------------------------------------------------
-  int b = -1, tile = blockIdx.x, base = 0;
-  Kv4Rows rows{};
-  for (int i0 = 0; i0 < p.a.n; i0 += 32) {
-    int tiles = 0;
-    if (i0 + lane < p.a.n) {
-      const int begin = p.a.ind ? min(max(p.a.ind[i0 + lane], 0), p.a.T) : 0;
-      const int end = p.a.ind ? min(max(p.a.ind[i0 + lane + 1], begin), p.a.T) : 1;
-      tiles = ((end - begin) * p.rep + 7) / 8;
-    }
-    int sum = tiles;
-    for (int d = 1; d < 32; d *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += v;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, base + sum > tile);
-    if (past) {
-      const int k = __ffs(past) - 1;
-      b = i0 + k;
-      tile -= base + __shfl_sync(0xffffffffu, sum - tiles, k);
-      break;
-    }
-    base += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  if (b < 0) return;
-  rows = kv4_rows(p.c, p.a.slots, p.a.ind, b, p.a.T, p.status);
-  const int n_rows = (rows.end - rows.begin) * p.rep, first = rows.length - (rows.end - rows.begin);
-  // ---- queries ---------------------------------------------------------------------------------------------------------
-  Queries<D, NG> q;
-  const int my = tile * 8 + g;
-  const __half* qp = static_cast<const __half*>(p.a.Q) + (rows.begin + min(my, n_rows - 1) / p.rep) * p.a.ldq +
-                     (head * p.rep + min(my, n_rows - 1) % p.rep) * D;
-  float sums[NG] = {};
+      for (int i = 0; i < 4; i++) {
+        const float w = sees(u, k, i) ? exp2_approx(x[u][k][i] - s.m[2 * k + (i & 1)]) : 0.0f;
+        x[u][k][i] = w;
+        s.l[2 * k + (i & 1)] += w;
+      }
+  // ---- O^T += V^T P^T, and what the 8 of c - 8 comes to: the same product with 8 for every code ---------------------------
+  float eight[NT][NG][4];
 #pragma unroll
-  for (int j = 0; j < J; j++) {
-    const uint4 v = *reinterpret_cast<const uint4*>(qp + (4 * j + t) * 8);
-    // dims 0..7 of the word pair up as (0, 4), (2, 6) for the low nibbles' step and (1, 5), (3, 7) for the high ones'
-    q.b[2 * j][0] = __byte_perm(v.x, v.z, 0x5410);
-    q.b[2 * j][1] = __byte_perm(v.y, v.w, 0x5410);
-    q.b[2 * j + 1][0] = __byte_perm(v.x, v.z, 0x7632);
-    q.b[2 * j + 1][1] = __byte_perm(v.y, v.w, 0x7632);
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
+  for (int k = 0; k < NT; k++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 f = __half22float2(h[i]);
-      sums[j * NG / J] += f.x + f.y;
-    }
-  }
+    for (int grp = 0; grp < NG; grp++)
 #pragma unroll
-  for (int grp = 0; grp < NG; grp++) {
-    sums[grp] += __shfl_xor_sync(0xffffffffu, sums[grp], 1);
-    sums[grp] += __shfl_xor_sync(0xffffffffu, sums[grp], 2);
-    q.sum[0][grp] = __shfl_sync(0xffffffffu, sums[grp], 8 * t);
-    q.sum[1][grp] = __shfl_sync(0xffffffffu, sums[grp], 8 * t + 4);
-  }
-  // ---- what rows 2t and 2t + 1 see: tokens [lo, hi) ----------------------------------------------------------------------
-  int lo[2], hi[2];
+      for (int i = 0; i < 4; i++) eight[k][grp][i] = 0.0f;
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    const int row = tile * 8 + 2 * t + r;
-    const int pos = first + row / p.rep;
-    const bool is = row < n_rows;
-    hi[r] = is ? pos + 1 : 0;
-    lo[r] = is && p.a.window > 0 ? max(pos + 1 - p.a.window, 0) : 0;
-  }
-  const int last_row = min(tile * 8 + 7, n_rows - 1);
-  const int end = first + last_row / p.rep + 1;  // tokens that some row of this tile sees end here
-  const int start = p.a.window > 0 ? max(first + tile * 8 / p.rep + 1 - p.a.window, 0) : 0;
-  RowState<D, NG> s;
-#pragma unroll
-  for (int r = 0; r < 2; r++) {
-    s.m[r] = -INFINITY;
-    s.l[r] = 0.0f;
-#pragma unroll
-    for (int grp = 0; grp < NG; grp++) s.z[r][grp] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < D / 16; i++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) s.o[i][k] = 0.0f;
-  s.e = -24;
-  const float cs = p.a.scale * LOG2E;
-  const int page_units = 1 << (p.c.page_shift - 4);
-  for (int u = start / 16 + warp; u * 16 < end; u += AT_WARPS) {
-    const int page = kv4_page(p.c, rows.slot, u * 16, p.status);
-    if (page < 0) continue;
-    const uint8_t* unit = p.c.pages + page * p.c.page_bytes +
-                          (static_cast<long long>(head) * page_units + (u & (page_units - 1))) * UNIT;
-    kv4_tile<D, NG>(unit, u * 16, lo[0], hi[0], lo[1], hi[1], cs, q, s);
-  }
-  // ---- join ------------------------------------------------------------------------------------------------------------
-#pragma unroll
-  for (int r = 0; r < 2; r++) {
-    s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 4);
-    s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 8);
-    s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 16);
+  for (int u = 0; u < UN; u++) {
+    const uint8_t* unit = stage + u * UNIT;
+    uint32_t vw0[J], vw1[J];
+    load_words<J>(vw0, unit + 8 * D + lane * W);
+    load_words<J>(vw1, unit + 12 * D + lane * W);
 #pragma unroll
     for (int grp = 0; grp < NG; grp++) {
-      s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 4);
-      s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 8);
-      s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 16);
+      uint32_t b0[NT], b1[NT];
+      const float2 va = __half22float2(*reinterpret_cast<const __half2*>(&vpar[u][0][grp]));
+      const float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&vpar[u][1][grp]));
+      const float za = fmaf(va.x, 8.0f, va.y), zb = fmaf(vb.x, 8.0f, vb.y), sa = va.x * up, sb = vb.x * up;
+#pragma unroll
+      for (int k = 0; k < NT; k++) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const bool see = sees(u, k, i);
+          w[i] = see ? x[u][k][i] * (i < 2 ? sa : sb) : 0.0f;
+          if (see) s.z[2 * k + (i & 1)][grp] = fmaf(x[u][k][i], i < 2 ? za : zb, s.z[2 * k + (i & 1)][grp]);
+        }
+        b0[k] = transpose_8x8(pack_half2(w[0], w[1]));
+        b1[k] = transpose_8x8(pack_half2(w[2], w[3]));
+      }
+#pragma unroll
+      for (int i = grp * J / NG; i < (grp + 1) * J / NG; i++) {
+        const uint32_t a = vw0[i], b = vw1[i], a2 = a >> 8, b2 = b >> 8;
+#pragma unroll
+        for (int k = 0; k < NT; k++) {
+          mma_16816(s.o[k][2 * i], a & Q4_LO, a2 & Q4_LO, b & Q4_LO, b2 & Q4_LO, b0[k], b1[k]);
+          mma_16816(s.o[k][2 * i + 1], a & Q4_HI, a2 & Q4_HI, b & Q4_HI, b2 & Q4_HI, b0[k], b1[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < NT; k++) mma_16816(eight[k][grp], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0[k], b1[k]);
     }
-    const float down = pow2i(s.e - 14);
+  }
+#pragma unroll
+  for (int k = 0; k < NT; k++)
 #pragma unroll
     for (int i = 0; i < J; i++)
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const float zero = s.z[r][i * NG / J];
-        so[warp][2 * t + r][32 * i + 4 * g + 2 * k] = fmaf(s.o[2 * i][2 * k + r] * Q4_LO_UNIT, down, zero);
-        so[warp][2 * t + r][32 * i + 4 * g + 2 * k + 1] = fmaf(s.o[2 * i + 1][2 * k + r] * Q4_HI_UNIT, down, zero);
+      for (int c = 0; c < 4; c++) {
+        s.o[k][2 * i][c] -= eight[k][i * NG / J][c];
+        s.o[k][2 * i + 1][c] = fmaf(-16.0f, eight[k][i * NG / J][c], s.o[k][2 * i + 1][c]);
       }
-    if (g == 0) {
-      sm[warp][2 * t + r] = s.m[r];
-      sl[warp][2 * t + r] = s.l[r];
+}
+
+template <int D, int NG, int NT, int UN, int STAGES>
+struct AttnShape {
+  static constexpr int ROWS = 8 * NT, UNIT = kv4_unit_bytes(D, D / NG), STAGE = UN * UNIT, RING = STAGES * STAGE;
+  static constexpr int PITCH = D + 4;  // of a row of partial o in shared memory
+  static constexpr int JOIN = AT_WARPS * ROWS * (PITCH + 2) * 4;
+  static constexpr int DATA = AT_WARPS * RING > JOIN ? AT_WARPS * RING : JOIN;
+  static constexpr int HEAD = 256;     // barriers, abort flag, sums
+  static constexpr int SMEM = HEAD + DATA;
+  static constexpr int PART = ROWS * (D + 2);  // floats of a part in the workspace: o, m, l
+};
+
+template <int D, int NG, int NT, int UN, int STAGES>
+__global__ void __launch_bounds__(AT_WARPS * 32) kv4_attn_kernel(AttnParams p) {
+  using S = AttnShape<D, NG, NT, UN, STAGES>;
+  constexpr int J = D / 32, ROWS = S::ROWS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);                 // [AT_WARPS][STAGES]
+  uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + 192);
+  static_assert(AT_WARPS * STAGES * 8 <= 192 && 196 <= S::HEAD, "shared memory head");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + S::HEAD + warp * S::RING;
+  uint64_t* bar = bars + warp * STAGES;
+  if (threadIdx.x < AT_WARPS * STAGES) mbar_init(bars + threadIdx.x, 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_mbar_init();
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long line = line_length<ROWS>(p);
+  __syncthreads();  // the barriers are set up
+  const long long piece = max((line + gridDim.x - 1) / gridDim.x, static_cast<long long>(AT_PIECE));
+  long long at = piece * blockIdx.x;
+  const long long stop = min(at + piece, line);
+  if (threadIdx.x == 0) p.cuts[blockIdx.x].parts = 0;
+  const WaitCtx ctx{abort_flag, p.status};
+  const float cq = p.a.scale * LOG2E, cs = cq * Q4_LO_UNIT;
+  const int page_units = 1 << (p.c.page_shift - 4);
+  int seq = 0;
+  long long seq_at = 0;
+  uint32_t phase = 0;  // tiles this warp has taken from its ring so far
+  while (at < stop) {
+    // ---- the problem at `at`, and how much of it lies in this piece -------------------------------------------------------
+    if (!find_sequence<ROWS>(p, at, &seq, &seq_at)) break;
+    Problem pr;
+    pr.rows = kv4_rows(p.c, p.a.slots, p.a.ind, seq, p.a.T, p.status);
+    pr.units = seq_units(p, pr.rows, &pr.u_begin);
+    const int span = pr.units + AT_START;
+    const long long index = (at - seq_at) / span;
+    const int tiles = seq_problems<ROWS>(p, pr.rows) / p.c.heads;
+    pr.head = static_cast<int>(index / tiles);
+    pr.tile = static_cast<int>(index % tiles);
+    const long long start = seq_at + index * span;  // of the problem, on the line
+    const bool continued = at > start;
+    const int from = max(static_cast<int>(at - start) - AT_START, 0);
+    const int upto = max(static_cast<int>(min(static_cast<long long>(span), stop - start)) - AT_START, 0);
+    if (threadIdx.x == 0 && !continued && start + span > stop) {
+      // pieces [lo, hi] hold its units: this one does not if it ends among the empty places
+      const long long lo = (start + AT_START) / piece, hi = (start + span - 1) / piece;
+      Cut cut;
+      cut.parts = hi > lo ? static_cast<int>(hi - lo) + 1 : 0;
+      cut.first = static_cast<int>(lo * 2 + (lo == blockIdx.x ? 1 : 0));
+      cut.next = static_cast<int>(lo * 2 + 2);
+      cut.row_begin = pr.rows.begin;
+      cut.n_rows = (pr.rows.end - pr.rows.begin) * p.rep;
+      cut.head = pr.head;
+      cut.tile = pr.tile;
+      cut.unused = 0;
+      p.cuts[blockIdx.x] = cut;
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 8 * D; i += AT_WARPS * 32) {
-    const int r = i / D, d = i % D, row = tile * 8 + r;
-    if (row >= n_rows) break;
-    float m = sm[0][r];
-    for (int w = 1; w < AT_WARPS; w++) m = fmaxf(m, sm[w][r]);
-    float l = 0.0f, o = 0.0f;
-    for (int w = 0; w < AT_WARPS; w++) {
-      const float f = sm[w][r] == -INFINITY ? 0.0f : exp2_approx(sm[w][r] - m);
-      l = fmaf(sl[w][r], f, l);
-      if (f != 0.0f) o = fmaf(so[w][r][d], f, o);
+    at = min(start + span, stop);
+    if (from >= upto) continue;                     // the piece ends among the problem's empty places
+    const bool whole = from == 0 && upto == pr.units;
+    const int u0 = pr.u_begin + from, u1 = pr.u_begin + upto;
+    const int n_rows = (pr.rows.end - pr.rows.begin) * p.rep, first = pr.rows.length - (pr.rows.end - pr.rows.begin);
+    // ---- this warp's units, their pages, and the first tiles under way ------------------------------------------------------
+    const int end_row = min(pr.tile * ROWS + ROWS - 1, n_rows - 1);
+    const int visible = (max(first + end_row / p.rep + 1, 0) + KV4_UNIT - 1) / KV4_UNIT;  // units that hold a seen token
+    const int v1 = max(min(u1, visible), u0), len = v1 - u0;
+    const int w0 = u0 + static_cast<int>(static_cast<long long>(len) * warp / AT_WARPS);
+    const int w1 = u0 + static_cast<int>(static_cast<long long>(len) * (warp + 1) / AT_WARPS);
+    int page_base = w0, page_id = -1;  // lane i knows the page of unit page_base + i
+    auto look_up = [&](int base) {
+      page_base = base;
+      page_id = base + lane < w1 ? kv4_page(p.c, pr.rows.slot, (base + lane) * KV4_UNIT, p.status) : -1;
+    };
+    auto issue = [&](int u, uint32_t at_tile) {  // units [u, u + UN) into the tile's stage; returns which are there
+      if (u + UN > page_base + 32) look_up(u);
+      const int page = __shfl_sync(0xffffffffu, page_id, (u - page_base + lane) & 31);
+      const bool is = lane < UN && u + lane < w1 && page >= 0;
+      const uint32_t present = __ballot_sync(0xffffffffu, is);
+      const int st = at_tile % STAGES;
+      if (lane == 0) mbar_arrive_expect_tx(bar + st, __popc(present) * S::UNIT);
+      __syncwarp();
+      if (is)
+        bulk_load(ring + st * S::STAGE + lane * S::UNIT,
+                  p.c.pages + page * p.c.page_bytes +
+                      (static_cast<long long>(pr.head) * page_units + ((u + lane) & (page_units - 1))) * S::UNIT,
+                  S::UNIT, bar + st);
+      return present;
+    };
+    if (w0 < w1) look_up(w0);
+    const int n_tiles = (w1 - w0 + UN - 1) / UN;
+    uint32_t present = 0;  // UN bits a stage
+    for (int k = 0; k < STAGES && k < n_tiles; k++) present |= issue(w0 + k * UN, phase + k) << ((phase + k) % STAGES * UN);
+    // ---- queries ---------------------------------------------------------------------------------------------------------
+    Queries<D, NG, NT> q;
+#pragma unroll
+    for (int k = 0; k < NT; k++) {
+      const int row = min(pr.tile * ROWS + k * 8 + g, n_rows - 1);
+      const __half* qp = static_cast<const __half*>(p.a.Q) + (pr.rows.begin + row / p.rep) * p.a.ldq +
+                         (pr.head * p.rep + row % p.rep) * D;
+      float sum[NG] = {};
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const uint4 v = *reinterpret_cast<const uint4*>(qp + (4 * j + t) * 8);
+        // dims 0..7 of the word pair up as (0, 4), (2, 6) for the low nibbles' step and (1, 5), (3, 7) for the high ones'
+        q.b[k][2 * j][0] = __byte_perm(v.x, v.z, 0x5410);
+        q.b[k][2 * j][1] = __byte_perm(v.y, v.w, 0x5410);
+        q.b[k][2 * j + 1][0] = __byte_perm(v.x, v.z, 0x7632);
+        q.b[k][2 * j + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float2 f = __half22float2(h[i]);
+          sum[j * NG / J] += f.x + f.y;
+        }
+      }
+#pragma unroll
+      for (int grp = 0; grp < NG; grp++) {
+        sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 1);
+        sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 2);
+        q.sum[2 * k][grp] = __shfl_sync(0xffffffffu, sum[grp], 8 * t) * cq;
+        q.sum[2 * k + 1][grp] = __shfl_sync(0xffffffffu, sum[grp], 8 * t + 4) * cq;
+      }
     }
-    const long long out = rows.begin + row / p.rep;
-    const int h = head * p.rep + row % p.rep;
-    static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(m == -INFINITY ? 0.0f : o / l);
-    if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = m == -INFINITY ? -INFINITY : fmaf(m, LN2, logf(l));
+#pragma unroll
+    for (int r = 0; r < 2 * NT; r++) {  // rows behind the last repeat it
+      const int pos = first + min(pr.tile * ROWS + (r >> 1) * 8 + 2 * t + (r & 1), n_rows - 1) / p.rep;
+      q.hi[r] = pos + 1;
+      q.lo[r] = p.a.window > 0 ? max(pos + 1 - p.a.window, 0) : 0;
+    }
+    // every row sees tokens [all_lo, all_hi)
+    const int all_hi = first + pr.tile * ROWS / p.rep + 1;
+    const int all_lo = p.a.window > 0 ? max(first + end_row / p.rep + 1 - p.a.window, 0) : 0;
+    RowState<D, NG, NT> s;
+#pragma unroll
+    for (int r = 0; r < 2 * NT; r++) {
+      s.m[r] = -INFINITY;
+      s.l[r] = 0.0f;
+#pragma unroll
+      for (int grp = 0; grp < NG; grp++) s.z[r][grp] = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < NT; k++)
+#pragma unroll
+      for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) s.o[k][i][c] = 0.0f;
+    s.e = -14;
+    // ---- tokens ------------------------------------------------------------------------------------------------------------
+#pragma unroll 1
+    for (int i = 0; i < n_tiles; i++) {
+      const uint32_t n = phase + i, st = n % STAGES, here = (present >> (st * UN)) & ((1u << UN) - 1);
+      if (!mbar_wait_warp(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx)) continue;  // recorded; nothing hangs
+      const int tok0 = (w0 + i * UN) * KV4_UNIT;
+      const uint8_t* stage = ring + st * S::STAGE;
+      if (tok0 >= all_lo && tok0 + UN * KV4_UNIT <= all_hi && here == (1u << UN) - 1)
+        kv4_tile<D, NG, NT, UN, false>(stage, tok0, here, cs, q, s);
+      else
+        kv4_tile<D, NG, NT, UN, true>(stage, tok0, here, cs, q, s);
+      __syncwarp();
+      if (i + STAGES < n_tiles) {
+        present &= ~(((1u << UN) - 1) << (st * UN));
+        present |= issue(w0 + (i + STAGES) * UN, n + STAGES) << (st * UN);
+      }
+    }
+    phase += n_tiles;
+    // ---- join the warps -----------------------------------------------------------------------------------------------------
+    float* so = reinterpret_cast<float*>(smem + S::HEAD);               // [AT_WARPS][ROWS][PITCH], m and l behind a row's o
+    __syncthreads();                                                    // every ring is drained
+#pragma unroll
+    for (int r = 0; r < 2 * NT; r++) {
+      const int row = (r >> 1) * 8 + 2 * t + (r & 1);
+      float* mine = so + (warp * ROWS + row) * (S::PITCH + 2);
+      s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 4);
+      s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 8);
+      s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 16);
+      const float down = pow2i(s.e - 14);
+#pragma unroll
+      for (int grp = 0; grp < NG; grp++) {
+        s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 4);
+        s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 8);
+        s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 16);
+      }
+#pragma unroll
+      for (int i = 0; i < J; i++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const float zero = s.z[r][i * NG / J];
+          mine[32 * i + 4 * g + 2 * k] = fmaf(s.o[r >> 1][2 * i][2 * k + (r & 1)] * Q4_LO_UNIT, down, zero);
+          mine[32 * i + 4 * g + 2 * k + 1] = fmaf(s.o[r >> 1][2 * i + 1][2 * k + (r & 1)] * Q4_HI_UNIT, down, zero);
+        }
+      if (g == 0) {
+        mine[S::PITCH] = s.m[r];
+        mine[S::PITCH + 1] = s.l[r];
+      }
+    }
+    __syncthreads();
+    float* part = p.part + (static_cast<long long>(blockIdx.x) * 2 + (continued ? 0 : 1)) * S::PART;
+    for (int i = threadIdx.x; i < ROWS * D; i += AT_WARPS * 32) {
+      const int r = i / D, d = i % D, row = pr.tile * ROWS + r;
+      if (row >= n_rows) break;
+      const float* one = so + r * (S::PITCH + 2);
+      constexpr int STEP = ROWS * (S::PITCH + 2);
+      float m = one[S::PITCH];
+#pragma unroll
+      for (int w = 1; w < AT_WARPS; w++) m = fmaxf(m, one[w * STEP + S::PITCH]);
+      float l = 0.0f, o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < AT_WARPS; w++) {
+        const float mw = one[w * STEP + S::PITCH], lw = one[w * STEP + S::PITCH + 1];
+        if (lw == 0.0f) continue;  // saw nothing (a NaN sum is kept)
+        const float f = exp2_approx(mw - m);
+        l = fmaf(lw, f, l);
+        o = fmaf(one[w * STEP + d], f, o);
+      }
+      if (whole) {
+        const long long out = pr.rows.begin + row / p.rep;
+        const int h = pr.head * p.rep + row % p.rep;
+        static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
+        if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
+      } else {
+        part[i] = o;
+        if (d == 0) {
+          part[ROWS * D + r] = m;
+          part[ROWS * D + ROWS + r] = l;
+        }
+      }
+    }
+    fence_proxy_async_smem();  // the next tiles' copies come after what was read and written here
+    __syncthreads();
   }
 }
 
+constexpr int JOIN_THREADS = 256;
+
+// Joins the parts of problems that were cut: CTA (c, r) takes row r of the problem that piece c left to be joined.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p) {
+  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, CHUNK = 256;
+  __shared__ float weight[CHUNK], top[JOIN_THREADS / 32], so[GROUPS][D], sl[JOIN_THREADS / 32];
+  pdl_wait();
+  const Cut cut = p.cuts[blockIdx.x];
+  const int r = blockIdx.y, row = cut.tile * ROWS + r, n = cut.parts;
+  if (n == 0 || row >= cut.n_rows) return;
+  auto part_of = [&](int i) { return p.part + static_cast<long long>(i == 0 ? cut.first : cut.next + 2 * (i - 1)) * PART; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x % D, group = threadIdx.x / D;
+  // the largest maximum, then every part's weight
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += JOIN_THREADS) m = fmaxf(m, part_of(i)[ROWS * D + r]);
+#pragma unroll
+  for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+  if (lane == 0) top[warp] = m;
+  __syncthreads();
+  for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, top[w]);
+  float l = 0.0f, o = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += CHUNK) {
+    const int i = i0 + threadIdx.x;
+    if (i < n) {
+      const float* part = part_of(i);
+      const float mi = part[ROWS * D + r], li = part[ROWS * D + ROWS + r];
+      const float f = li == 0.0f ? 0.0f : exp2_approx(mi - m);  // (a part that saw nothing holds no numbers)
+      weight[threadIdx.x] = f;
+      if (li != 0.0f) l = fmaf(li, f, l);
+    }
+    __syncthreads();
+    const int end = min(n - i0, CHUNK);
+#pragma unroll 8
+    for (int k = group; k < end; k += GROUPS) {
+      const float f = weight[k], v = part_of(i0 + k)[r * D + d];
+      o = f == 0.0f ? o : fmaf(v, f, o);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k /= 2) l += __shfl_xor_sync(0xffffffffu, l, k);
+  if (lane == 0) sl[warp] = l;
+  so[group][d] = o;
+  __syncthreads();
+  if (group != 0) return;
+  l = o = 0.0f;
+  for (int w = 0; w < JOIN_THREADS / 32; w++) l += sl[w];
+  for (int k = 0; k < GROUPS; k++) o += so[k][d];
+  const long long out = cut.row_begin + row / p.rep;
+  const int h = cut.head * p.rep + row % p.rep;
+  static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
+  if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
+}
+
+constexpr int AT_MOST_PER_SM = 4;
+
+// CTAs of a kernel that share an SM, asked for once per device.
+template <int D, int NG, int NT, int UN, int STAGES>
+cudaError_t per_sm_of(int* per_sm) {
+  constexpr int smem = AttnShape<D, NG, NT, UN, STAGES>::SMEM;
+  auto kernel = kv4_attn_kernel<D, NG, NT, UN, STAGES>;
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  *per_sm = dev < 64 ? known[dev].load(std::memory_order_acquire) : 0;
+  if (*per_sm > 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kernel, AT_WARPS * 32, smem);
+  if (e != cudaSuccess) return e;
+  *per_sm = *per_sm < 1 ? 1 : *per_sm > AT_MOST_PER_SM ? AT_MOST_PER_SM : *per_sm;
+  if (dev < 64) known[dev].store(*per_sm, std::memory_order_release);
+  return cudaSuccess;
+}
+
+template <int D, int NG, int NT, int UN, int STAGES>
+cudaError_t launch_attn(AttnParams& p, int most_rows, int sm_count, cudaStream_t stream) {
+  using S = AttnShape<D, NG, NT, UN, STAGES>;
+  auto kernel = kv4_attn_kernel<D, NG, NT, UN, STAGES>;
+  int per_sm = 0;
+  cudaError_t e = per_sm_of<D, NG, NT, UN, STAGES>(&per_sm);
+  if (e != cudaSuccess) return e;
+  p.pieces = sm_count * per_sm;
+  e = launch_with_pdl(kernel, dim3(p.pieces), dim3(AT_WARPS * 32), S::SMEM, stream, p);
+  if (e != cudaSuccess) return e;
+  if (p.pieces == 1) return cudaSuccess;
+  const dim3 cuts(p.pieces - 1, min(most_rows, S::ROWS));
+  return launch_with_pdl(kv4_join_kernel<D, S::ROWS>, cuts, dim3(JOIN_THREADS), 0, stream, p);
+}
+
+template <int D, int NG>
+cudaError_t launch_rows_of(AttnParams& p, int nt, int most_rows, int sm_count, cudaStream_t stream) {
+  return nt == 1 ? launch_attn<D, NG, 1, 4, 2>(p, most_rows, sm_count, stream) : launch_attn<D, NG, 2, 2, 3>(p, most_rows, sm_count, stream);
+}
+
+// Rows of a problem: eight where every sequence brings at most eight rows a key/value head, sixteen otherwise.
+int row_tiles(const Kv4View& c, int T, int n, int q_heads, bool one_each) { return q_heads / c.heads > 8 || (!one_each && T > n) ? 2 : 1; }
+
 }  // namespace
 
-size_t kv4_attention_workspace(const Kv4View& c, int T, int n, int q_heads, int sm_count) { return 0; }
+size_t kv4_attention_workspace(const Kv4View& c, int T, int n, int q_heads, int sm_count) {
+  return static_cast<size_t>(sm_count) * AT_MOST_PER_SM * (sizeof(Cut) + 2 * (16 * (c.D + 2)) * sizeof(float));
+}
 
 int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, size_t workspace_bytes, int sm_count,
                          uint32_t* status, cudaStream_t stream, const char** err) {
-  AttnParams p{c, a, a.q_heads / c.heads, status};
-  const long long tiles = a.ind ? (static_cast<long long>(a.T) * p.rep + 7) / 8 + a.n
-                                : static_cast<long long>(a.n) * ((p.rep + 7) / 8);
-  if (tiles > 0x7fffffffLL || c.heads > 65535) {
-    *err = "kv4_attention: too many rows";
-    return -2;
-  }
-  const dim3 grid(static_cast<unsigned>(tiles), c.heads);
+  Cut* cuts = static_cast<Cut*>(workspace);
+  AttnParams p{c, a, a.q_heads / c.heads, 0, cuts, reinterpret_cast<float*>(cuts + sm_count * AT_MOST_PER_SM), status};
+  const int nt = row_tiles(c, a.T, a.n, a.q_heads, a.ind == nullptr);
+  const int most_rows = a.ind ? 8 * nt : p.rep;  // rows of a problem that can be there
   const int ng = c.D / c.G;
-  if (c.D == 128) {
-    if (ng == 1) kv4_attn_kernel<128, 1><<<grid, AT_WARPS * 32, 0, stream>>>(p);
-    else if (ng == 2) kv4_attn_kernel<128, 2><<<grid, AT_WARPS * 32, 0, stream>>>(p);
-    else kv4_attn_kernel<128, 4><<<grid, AT_WARPS * 32, 0, stream>>>(p);
-  } else {
-    if (ng == 1) kv4_attn_kernel<64, 1><<<grid, AT_WARPS * 32, 0, stream>>>(p);
-    else kv4_attn_kernel<64, 2><<<grid, AT_WARPS * 32, 0, stream>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (c.D == 128)
+    e = ng == 1 ? launch_rows_of<128, 1>(p, nt, most_rows, sm_count, stream)
+      : ng == 2 ? launch_rows_of<128, 2>(p, nt, most_rows, sm_count, stream)
+                : launch_rows_of<128, 4>(p, nt, most_rows, sm_count, stream);
+  else
+    e = ng == 1 ? launch_rows_of<64, 1>(p, nt, most_rows, sm_count, stream) : launch_rows_of<64, 2>(p, nt, most_rows, sm_count, stream);
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess) return 0;
   *err = cudaGetErrorString(e);
   return -3;

@@ -14,8 +14,9 @@ Calls enqueue on the current (or given) stream; index arrays are int32 device te
 from __future__ import annotations
 
 import ctypes
+import struct
 
-from . import (F16, F32, I8, I32, PH_ERR_INVALID, PH_ERR_UNSUPPORTED, PhobosError, PhTensor, _stream_ptr, _ws, check, lib)
+from . import (F16, F32, I8, I32, PH_ERR_INVALID, PH_ERR_UNSUPPORTED, PhobosError, PhTensor, check, lib)
 
 
 class PhKv4Cache(ctypes.Structure):
@@ -25,41 +26,80 @@ class PhKv4Cache(ctypes.Structure):
                 ("group", ctypes.c_int32), ("max_seqs", ctypes.c_int32), ("table_width", ctypes.c_int32)]
 
 
-def _on_device(t, name: str) -> None:
-    import torch
-    if not t.is_cuda:
-        raise PhobosError(PH_ERR_INVALID, f"{name} is not on a CUDA device")
-    if t.device.index != torch.cuda.current_device():
-        raise PhobosError(PH_ERR_INVALID, f"{name} lives on cuda:{t.device.index} but the current device is "
-                                          f"cuda:{torch.cuda.current_device()}")
+_PACK = struct.Struct("<Qiiqqqqq").pack     # PhTensor, as the C compiler lays it out
+assert struct.calcsize("<Qiiqqqqq") == ctypes.sizeof(PhTensor)
 
 
-def _desc(t, name: str) -> PhTensor:
-    """PhTensor of a rank-1/2 CUDA tensor of any element type these entry points know (no copy)."""
+def _codes():
     import torch
-    _on_device(t, name)
-    codes = {torch.float16: F16, torch.float32: F32, torch.int8: I8, torch.uint8: I8, torch.int32: I32}
-    if t.dtype not in codes:
+    return {torch.float16: F16, torch.float32: F32, torch.int8: I8, torch.uint8: I8, torch.int32: I32}
+
+
+def _device() -> int:
+    import torch
+    return torch.cuda.current_device()
+
+
+def _stream(stream, device: int) -> int:
+    """The stream's handle.  (The raw handle of the current one costs a tenth of what building a Stream object does, which
+    is much of a short call.)"""
+    if stream is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _on_device(t, name: str, device: int) -> None:
+    if t.get_device() != device:      # -1 for a CPU tensor
+        if not t.is_cuda:
+            raise PhobosError(PH_ERR_INVALID, f"{name} is not on a CUDA device")
+        raise PhobosError(PH_ERR_INVALID, f"{name} lives on cuda:{t.device.index} but the current device is cuda:{device}")
+
+
+def _desc(t, name: str, device: int) -> bytes:
+    """A PhTensor, as bytes, of a rank-1/2 CUDA tensor of any element type these entry points know (no copy)."""
+    global _CODES
+    if _CODES is None:
+        _CODES = _codes()
+    _on_device(t, name, device)
+    code = _CODES.get(t.dtype)
+    if code is None:
         raise PhobosError(PH_ERR_UNSUPPORTED, f"{name}: element type {t.dtype}")
-    if t.dim() not in (1, 2):
-        raise PhobosError(PH_ERR_INVALID, f"{name}: rank {t.dim()}, expected 1 or 2")
-    d = PhTensor(t.data_ptr(), codes[t.dtype], t.dim())
-    for i in range(t.dim()):
-        d.sizes[i], d.strides[i] = t.shape[i], t.stride(i)
-    return d
+    size, stride = t.shape, t.stride()
+    if len(size) == 2:
+        return _PACK(t.data_ptr(), code, 2, size[0], size[1], stride[0], stride[1], 0)
+    if len(size) == 1:
+        return _PACK(t.data_ptr(), code, 1, size[0], 0, stride[0], 0, 0)
+    raise PhobosError(PH_ERR_INVALID, f"{name}: rank {len(size)}, expected 1 or 2")
 
 
-def _ints(t, name: str, n: int | None = None):
+_CODES = None
+
+
+def byte_desc(t) -> PhTensor:
+    """The descriptor of `launch` for a tensor that is not f16 or f32."""
+    return PhTensor.from_buffer_copy(_desc(t, "tensor", _device()))
+
+
+def _ints(t, name: str, device: int, n: int = 0):
     """Address of a contiguous int32 device tensor of at least n values (None stays None)."""
-    import torch
     if t is None:
         return None
-    _on_device(t, name)
-    if t.dtype != torch.int32 or not t.is_contiguous():
+    _on_device(t, name, device)
+    import torch
+    if t.dtype is not torch.int32 or not t.is_contiguous():
         raise PhobosError(PH_ERR_INVALID, f"{name}: expected a contiguous int32 tensor")
-    if n is not None and t.numel() < n:
+    if t.numel() < n:
         raise PhobosError(PH_ERR_INVALID, f"{name}: {t.numel()} values, expected {n}")
     return t.data_ptr()
+
+
+def _space(workspace, device: int):
+    if workspace is None:
+        return None, 0
+    _on_device(workspace, "workspace", device)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 # ---- 4-bit weights ----------------------------------------------------------------------------
@@ -73,17 +113,18 @@ def q4_pack(codes, scales, zeros, group: int, out=None, stream=None):
     if out is None:
         need = q4_packed_bytes(codes.shape[0], codes.shape[1], group)
         out = torch.empty(need, dtype=torch.int8, device=codes.device)
-    c, s, o = _desc(codes, "codes"), _desc(scales, "scales"), _desc(out, "packed")
-    z = _desc(zeros, "zeros") if zeros is not None else None
-    check(lib().phobos_q4_pack(ctypes.byref(c), ctypes.byref(s), ctypes.byref(z) if z else None, group, ctypes.byref(o),
-                               _stream_ptr(stream)))
+    dev = _device()
+    z = _desc(zeros, "zeros", dev) if zeros is not None else None
+    check(lib().phobos_q4_pack(_desc(codes, "codes", dev), _desc(scales, "scales", dev), z, group, _desc(out, "packed", dev),
+                               _stream(stream, dev)))
     return out
 
 
 def gemv_q4(X, packed, Y, group: int, alpha: float = 1.0, beta: float = 0.0, stream=None) -> None:
     """Y[M,N] = alpha * X[M,K] W[N,K]^T + beta * Y, W = scale * (code - zero) in 4 bits; X f16, Y f16 or f32."""
-    x, w, y = _desc(X, "X"), _desc(packed, "packed"), _desc(Y, "Y")
-    check(lib().phobos_gemv_q4(ctypes.byref(x), ctypes.byref(w), ctypes.byref(y), alpha, beta, group, _stream_ptr(stream)))
+    dev = _device()
+    check(lib().phobos_gemv_q4(_desc(X, "X", dev), _desc(packed, "packed", dev), _desc(Y, "Y", dev), alpha, beta, group,
+                               _stream(stream, dev)))
 
 
 # ---- the cache ------------------------------------------------------------------------------------
@@ -96,8 +137,9 @@ class Kv4Cache:
     tables [max_seqs, table_width], lens [max_seqs].  Holds the tensors; the calls below change them in place."""
 
     def __init__(self, pages, refs, tables, lens, *, kv_heads: int, head_dim: int, group: int, page_tokens: int):
+        dev = _device()
         for t, name in ((pages, "pages"), (refs, "refs"), (tables, "tables"), (lens, "lens")):
-            _on_device(t, name)
+            _on_device(t, name, dev)
         need = kv4_page_bytes(kv_heads, head_dim, group, page_tokens)
         if need == 0:
             raise PhobosError(PH_ERR_UNSUPPORTED, f"kv4: {kv_heads} heads of {head_dim} dims in groups of {group}, pages of "
@@ -110,9 +152,10 @@ class Kv4Cache:
         self.pages, self.refs, self.tables, self.lens = pages, refs, tables, lens
         self.kv_heads, self.head_dim, self.group, self.page_tokens = kv_heads, head_dim, group, page_tokens
         pitch = pages.stride(0) if pages.shape[0] > 1 else 0
-        self.struct = PhKv4Cache(pages.data_ptr(), _ints(refs, "refs"), _ints(tables, "tables"), _ints(lens, "lens"), pitch,
+        self.struct = PhKv4Cache(pages.data_ptr(), _ints(refs, "refs", dev), _ints(tables, "tables", dev), _ints(lens, "lens", dev), pitch,
                                  pages.shape[0], pages.shape[1], page_tokens, kv_heads, head_dim, group, tables.shape[0],
                                  tables.shape[1])
+        self.address, self.device = ctypes.addressof(self.struct), dev
 
     @classmethod
     def create(cls, layers: int, n_pages: int, kv_heads: int, head_dim: int, group: int, page_tokens: int, max_seqs: int,
@@ -127,70 +170,69 @@ class Kv4Cache:
 
 
 def _batch(cache: Kv4Cache, slots, indptr):
-    _on_device(cache.pages, "the cache")
+    dev = _device()
+    if cache.device != dev:
+        raise PhobosError(PH_ERR_INVALID, f"the cache lives on cuda:{cache.device} but the current device is cuda:{dev}")
     n = slots.numel()
-    return _ints(slots, "slots"), _ints(indptr, "indptr", n + 1), n
+    return dev, _ints(slots, "slots", dev), _ints(indptr, "indptr", dev, n + 1), n
 
 
 def kv4_append(cache: Kv4Cache, layer: int, K, V, slots, indptr=None, stream=None) -> None:
     """Quantises rows K, V [T, kv_heads * head_dim] into the places of the sequences' last tokens (see kv4_extend)."""
-    s, i, n = _batch(cache, slots, indptr)
-    k, v = _desc(K, "K"), _desc(V, "V")
-    check(lib().phobos_kv4_append(ctypes.byref(cache.struct), layer, ctypes.byref(k), ctypes.byref(v), s, i, n, _stream_ptr(stream)))
+    dev, s, i, n = _batch(cache, slots, indptr)
+    check(lib().phobos_kv4_append(cache.address, layer, _desc(K, "K", dev), _desc(V, "V", dev), s, i, n, _stream(stream, dev)))
 
 
 def kv4_read(cache: Kv4Cache, layer: int, K, V, slots, indptr=None, stream=None) -> None:
     """The values of the sequences' last tokens into rows K, V: the inverse of kv4_append."""
-    s, i, n = _batch(cache, slots, indptr)
-    k, v = _desc(K, "K"), _desc(V, "V")
-    check(lib().phobos_kv4_read(ctypes.byref(cache.struct), layer, ctypes.byref(k), ctypes.byref(v), s, i, n, _stream_ptr(stream)))
+    dev, s, i, n = _batch(cache, slots, indptr)
+    check(lib().phobos_kv4_read(cache.address, layer, _desc(K, "K", dev), _desc(V, "V", dev), s, i, n, _stream(stream, dev)))
 
 
 def kv4_attention_workspace_bytes(cache: Kv4Cache, T: int, n: int, q_heads: int) -> int:
-    return int(lib().phobos_kv4_attention_workspace_bytes(ctypes.byref(cache.struct), T, n, q_heads))
+    return int(lib().phobos_kv4_attention_workspace_bytes(cache.address, T, n, q_heads))
 
 
 def kv4_attention(cache: Kv4Cache, layer: int, Q, O, scale: float, slots, indptr=None, lse=None, window: int = 0, workspace=None,
                   stream=None) -> None:
     """O = softmax(scale q K^T) V over the cache; Q, O [T, q_heads * head_dim] f16.  The row of position p sees tokens
     j <= p (window > 0: only j > p - window); one that sees nothing gets zeros and lse -inf."""
-    s, i, n = _batch(cache, slots, indptr)
-    q, o = _desc(Q, "Q"), _desc(O, "O")
-    l = _desc(lse, "lse") if lse is not None else None
-    wp, wn = _ws(workspace)
-    check(lib().phobos_kv4_attention(ctypes.byref(cache.struct), layer, ctypes.byref(q), ctypes.byref(o),
-                                     ctypes.byref(l) if l else None, scale, window, s, i, n, wp, wn, _stream_ptr(stream)))
+    dev, s, i, n = _batch(cache, slots, indptr)
+    l = _desc(lse, "lse", dev) if lse is not None else None
+    wp, wn = _space(workspace, dev)
+    check(lib().phobos_kv4_attention(cache.address, layer, _desc(Q, "Q", dev), _desc(O, "O", dev), l, scale, window, s, i, n, wp, wn,
+                                     _stream(stream, dev)))
 
 
 def kv4_pages_workspace_bytes(cache: Kv4Cache) -> int:
-    return int(lib().phobos_kv4_pages_workspace_bytes(ctypes.byref(cache.struct)))
+    return int(lib().phobos_kv4_pages_workspace_bytes(cache.address))
 
 
 def kv4_extend(cache: Kv4Cache, slots, counts, shortfall, workspace=None, stream=None) -> None:
     """Room for counts[i] more tokens of slots[i], and the new lengths.  shortfall (int32 [1], device): 0 done, > 0 pages
     missing, -1 a wrong request; unless it is 0 nothing has changed and the rows must not be appended."""
-    s, _, n = _batch(cache, slots, None)
-    wp, wn = _ws(workspace)
-    check(lib().phobos_kv4_extend(ctypes.byref(cache.struct), s, _ints(counts, "counts", n), n, _ints(shortfall, "shortfall", 1), wp, wn,
-                                  _stream_ptr(stream)))
+    dev, s, _, n = _batch(cache, slots, None)
+    wp, wn = _space(workspace, dev)
+    check(lib().phobos_kv4_extend(cache.address, s, _ints(counts, "counts", dev, n), n, _ints(shortfall, "shortfall", dev, 1), wp, wn,
+                                  _stream(stream, dev)))
 
 
 def kv4_fork(cache: Kv4Cache, src, dst, shortfall, deep: bool = False, workspace=None, stream=None) -> None:
     """The empty sequences dst[i] continue from src[i], sharing its pages, or (deep) with copies of them."""
-    s, _, n = _batch(cache, src, None)
-    wp, wn = _ws(workspace)
-    check(lib().phobos_kv4_fork(ctypes.byref(cache.struct), s, _ints(dst, "dst", n), n, int(deep), _ints(shortfall, "shortfall", 1), wp, wn,
-                                _stream_ptr(stream)))
+    dev, s, _, n = _batch(cache, src, None)
+    wp, wn = _space(workspace, dev)
+    check(lib().phobos_kv4_fork(cache.address, s, _ints(dst, "dst", dev, n), n, int(deep), _ints(shortfall, "shortfall", dev, 1), wp, wn,
+                                _stream(stream, dev)))
 
 
 def kv4_free(cache: Kv4Cache, slots, keep=None, stream=None) -> None:
     """Shortens slots[i] to keep[i] tokens (None: to none) and gives the pages behind them back."""
-    s, _, n = _batch(cache, slots, None)
-    check(lib().phobos_kv4_free(ctypes.byref(cache.struct), s, _ints(keep, "keep", n), n, _stream_ptr(stream)))
+    dev, s, _, n = _batch(cache, slots, None)
+    check(lib().phobos_kv4_free(cache.address, s, _ints(keep, "keep", dev, n), n, _stream(stream, dev)))
 
 
 def kv4_compact(cache: Kv4Cache, live, workspace=None, stream=None) -> None:
     """Moves the pages in use to ids 0 .. live[0] - 1 in every layer."""
-    _on_device(cache.pages, "the cache")
-    wp, wn = _ws(workspace)
-    check(lib().phobos_kv4_compact(ctypes.byref(cache.struct), _ints(live, "live", 1), wp, wn, _stream_ptr(stream)))
+    dev, _, _, _ = _batch(cache, live, None)
+    wp, wn = _space(workspace, dev)
+    check(lib().phobos_kv4_compact(cache.address, _ints(live, "live", dev, 1), wp, wn, _stream(stream, dev)))

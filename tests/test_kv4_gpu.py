@@ -437,13 +437,15 @@ def test_refusals(ph, dev):
     s = Setup(ph, dev, [20], 2, 64, 64, 16)
     q = torch.randn(1, 256, device=dev).half()
     kv = torch.randn(1, 128, device=dev).half()
-    ws = torch.empty(1 << 22, dtype=torch.uint8, device=dev)
+    need = ph.kv4_attention_workspace_bytes(s.cache, 1, 1, 4)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device=dev)
     att = lambda **k: ph.kv4_attention(s.cache, k.get("layer", 0), k.get("q", q), k.get("o", torch.empty_like(k.get("q", q))), 0.1, k.get("slots", s.slots),  # noqa: E731
                                        k.get("ind"), lse=k.get("lse"), window=k.get("window", 0), workspace=k.get("ws", ws))
     bad = [lambda: att(layer=1), lambda: att(layer=-1), lambda: att(q=q.float()), lambda: att(q=q[:, :192]), lambda: att(o=torch.empty(2, 256, device=dev).half()),
            lambda: att(window=-1), lambda: att(slots=s.slots.long()), lambda: att(slots=torch.zeros(2, dtype=torch.int32, device=dev)),
            lambda: att(lse=torch.empty(1, 3, device=dev)), lambda: att(lse=torch.empty(1, 4, device=dev).half()),
            lambda: att(ind=torch.zeros(1, dtype=torch.int32, device=dev)), lambda: att(q=torch.randn(1, 264, device=dev).half()[:, 4:260]),
+           lambda: att(ws=None), lambda: att(ws=ws[:need - 1]), lambda: att(ws=ws[8:]),
            lambda: ph.kv4_append(s.cache, 0, kv, kv[:, :64], s.slots), lambda: ph.kv4_append(s.cache, 0, kv.float(), kv.float(), s.slots),
            lambda: ph.kv4_append(s.cache, 3, kv, kv, s.slots), lambda: ph.kv4_read(s.cache, 0, kv[:0], kv, s.slots),
            lambda: ph.Kv4Cache.create(1, 4, 2, 96, 32, 16, 2, 4), lambda: ph.Kv4Cache.create(1, 4, 2, 64, 128, 16, 2, 4),
