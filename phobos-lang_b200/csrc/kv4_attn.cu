@@ -15,12 +15,11 @@
 //
 // Work: a problem is one sequence, one key/value head and 8 NT query rows (a row is one query token and one of the
 // heads that read the key/value head).  The units of 16 tokens of all problems form one line that is cut into equal
-// pieces, one per CTA; a CTA's warps cut each problem's part of the piece again.  On the line every problem stands
-// behind AT_START places that hold no units: what starting one costs, so that a piece of many short sequences is not
-// longer than one of a long sequence.  A problem whose units lie in one piece is finished there; one that was cut
-// leaves (m, l, o) of its parts in the workspace for a second, small kernel.
-// Each warp streams its units through a ring in shared memory with bulk copies (one per unit, 2176 bytes at D = G =
-// 128) that it issues itself: no barrier between warps while tokens last.
+// pieces, one per warp of a grid that fills the GPU once.  On the line every problem stands behind AT_START places that
+// hold no units: what starting one costs, so that a piece of many short sequences is not longer than one of a long
+// sequence.  A problem whose units lie in one piece is finished there; one that was cut leaves (m, l, o) of its parts in
+// the workspace for a second, small kernel.  Warps share nothing: each streams its units through a ring of its own in
+// shared memory with bulk copies (one per unit, 2176 bytes at D = G = 128) that it issues itself.
 #include <atomic>
 
 #include "kv4.cuh"
@@ -30,8 +29,9 @@ namespace ph {
 namespace {
 
 constexpr int AT_WARPS = 4;
-constexpr int AT_START = 16;             // places for starting a problem
-constexpr int AT_PIECE = AT_START + 16;  // a piece is at least that: a tile of four units for each warp
+constexpr int AT_START = 8;             // places for starting a problem
+constexpr int AT_PIECE = AT_START + 4;  // a piece is at least that long: one tile
+constexpr uint32_t EIGHT = 0x00080008u;  // 8 * 2^-24, as a low nibble's 8, two f16
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum : uint32_t { SITE_KV4_RING = 0x41 };
 
@@ -64,8 +64,8 @@ struct AttnParams {
   Kv4View c;
   Kv4AttnArgs a;
   int rep, pieces;
-  struct Cut* cuts;  // per CTA: the problem that its piece ends inside of
-  float* part;  // per CTA two parts: of the problem its piece begins inside of, and of the one it ends inside of
+  struct Cut* cuts;  // per piece: the problem that it ends inside of
+  float* part;       // per piece two parts: of the problem it begins inside of, and of the one it ends inside of
   uint32_t* status;
 };
 
@@ -74,14 +74,7 @@ struct Cut {
   int parts;          // 0: none, or its units lie in one piece
   int first;          // index of its first part in the workspace; the following ones are those that continue it in the
   int next;           // pieces after it: next, next + 2, ...
-  int row_begin, n_rows, head, tile, unused;
-};
-
-// One row tile of one sequence and key/value head, and where its units lie on the line.
-struct Problem {
-  Kv4Rows rows;
-  int head, tile;
-  int u_begin, units;      // tokens [16 u_begin, 16 (u_begin + units))
+  int row_begin, n_rows, head, row0, unused;
 };
 
 // Units of every problem of sequence b, and their first; at least one, so that rows without a token are answered too.
@@ -162,37 +155,47 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* stage, int tok0, uint32_
   const int lane = threadIdx.x & 31, g = lane >> 2;
   // ---- S^T -------------------------------------------------------------------------------------------------------
   float x[UN][NT][4];  // tokens g (0, 1) and g + 8 (2, 3), rows 2t and 2t + 1
+  constexpr int PAIR = UN % 2 == 0 ? 2 : 1;  // units whose matrix steps alternate: each unit's are a chain
 #pragma unroll
-  for (int u = 0; u < UN; u++) {
-    const uint8_t* unit = stage + u * UNIT;
-    uint32_t kw0[J], kw1[J];
-    load_words<J>(kw0, unit + lane * W);
-    load_words<J>(kw1, unit + 4 * D + lane * W);
-    const __half2* kpar = reinterpret_cast<const __half2*>(unit + 16 * D);
+  for (int u0 = 0; u0 < UN; u0 += PAIR) {
+    uint32_t kw0[PAIR][J], kw1[PAIR][J];
 #pragma unroll
-    for (int k = 0; k < NT; k++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) x[u][k][i] = 0.0f;
+    for (int v = 0; v < PAIR; v++) {
+      load_words<J>(kw0[v], stage + (u0 + v) * UNIT + lane * W);
+      load_words<J>(kw1[v], stage + (u0 + v) * UNIT + 4 * D + lane * W);
+    }
 #pragma unroll
     for (int grp = 0; grp < NG; grp++) {
-      float lo[NT][4] = {}, hi[NT][4] = {};
+      float lo[PAIR][NT][4], hi[PAIR][NT][4];
 #pragma unroll
-      for (int j = grp * J / NG; j < (grp + 1) * J / NG; j++) {
-        const uint32_t a = kw0[j], b = kw1[j], a2 = a >> 8, b2 = b >> 8;
+      for (int j = grp * J / NG; j < (grp + 1) * J / NG; j++)
 #pragma unroll
-        for (int k = 0; k < NT; k++) {
-          mma_16816(lo[k], a & Q4_LO, b & Q4_LO, a2 & Q4_LO, b2 & Q4_LO, q.b[k][2 * j][0], q.b[k][2 * j][1]);
-          mma_16816(hi[k], a & Q4_HI, b & Q4_HI, a2 & Q4_HI, b2 & Q4_HI, q.b[k][2 * j + 1][0], q.b[k][2 * j + 1][1]);
+        for (int v = 0; v < PAIR; v++) {
+          const uint32_t a = kw0[v][j], b = kw1[v][j], a2 = a >> 8, b2 = b >> 8;
+#pragma unroll
+          for (int k = 0; k < NT; k++) {
+            if (j == grp * J / NG) {
+              mma_16816_first(lo[v][k], a & Q4_LO, b & Q4_LO, a2 & Q4_LO, b2 & Q4_LO, q.b[k][2 * j][0], q.b[k][2 * j][1]);
+              mma_16816_first(hi[v][k], a & Q4_HI, b & Q4_HI, a2 & Q4_HI, b2 & Q4_HI, q.b[k][2 * j + 1][0], q.b[k][2 * j + 1][1]);
+            } else {
+              mma_16816(lo[v][k], a & Q4_LO, b & Q4_LO, a2 & Q4_LO, b2 & Q4_LO, q.b[k][2 * j][0], q.b[k][2 * j][1]);
+              mma_16816(hi[v][k], a & Q4_HI, b & Q4_HI, a2 & Q4_HI, b2 & Q4_HI, q.b[k][2 * j + 1][0], q.b[k][2 * j + 1][1]);
+            }
+          }
         }
+#pragma unroll
+      for (int v = 0; v < PAIR; v++) {
+        const __half2* kpar = reinterpret_cast<const __half2*>(stage + (u0 + v) * UNIT + 16 * D);
+        const float2 pa = __half22float2(kpar[g * NG + grp]), pb = __half22float2(kpar[(g + 8) * NG + grp]);
+        const float sa = pa.x * cs, sb = pb.x * cs;
+#pragma unroll
+        for (int k = 0; k < NT; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float dot = fmaf(hi[v][k][i], 1.0f / 16.0f, lo[v][k][i]), z = i < 2 ? pa.y : pb.y, qs = q.sum[2 * k + (i & 1)][grp];
+            x[u0 + v][k][i] = fmaf(i < 2 ? sa : sb, dot, grp == 0 ? z * qs : fmaf(z, qs, x[u0 + v][k][i]));
+          }
       }
-      const float2 pa = __half22float2(kpar[g * NG + grp]), pb = __half22float2(kpar[(g + 8) * NG + grp]);
-      const float sa = pa.x * cs, sb = pb.x * cs;
-#pragma unroll
-      for (int k = 0; k < NT; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          x[u][k][i] = fmaf(i < 2 ? sa : sb, fmaf(hi[k][i], 1.0f / 16.0f, lo[k][i]),
-                            fmaf(i < 2 ? pa.y : pb.y, q.sum[2 * k + (i & 1)][grp], x[u][k][i]));
     }
   }
   auto sees = [&](int u, int k, int i) {
@@ -271,12 +274,6 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* stage, int tok0, uint32_
   // ---- O^T += V^T P^T, and what the 8 of c - 8 comes to: the same product with 8 for every code ---------------------------
   float eight[NT][NG][4];
 #pragma unroll
-  for (int k = 0; k < NT; k++)
-#pragma unroll
-    for (int grp = 0; grp < NG; grp++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) eight[k][grp][i] = 0.0f;
-#pragma unroll
   for (int u = 0; u < UN; u++) {
     const uint8_t* unit = stage + u * UNIT;
     uint32_t vw0[J], vw1[J];
@@ -310,7 +307,12 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* stage, int tok0, uint32_
         }
       }
 #pragma unroll
-      for (int k = 0; k < NT; k++) mma_16816(eight[k][grp], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0[k], b1[k]);
+      for (int k = 0; k < NT; k++) {
+        if (u == 0)
+          mma_16816_first(eight[k][grp], EIGHT, EIGHT, EIGHT, EIGHT, b0[k], b1[k]);
+        else
+          mma_16816(eight[k][grp], EIGHT, EIGHT, EIGHT, EIGHT, b0[k], b1[k]);
+      }
     }
   }
 #pragma unroll
@@ -319,24 +321,21 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* stage, int tok0, uint32_
     for (int i = 0; i < J; i++)
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        s.o[k][2 * i][c] -= eight[k][i * NG / J][c];
-        s.o[k][2 * i + 1][c] = fmaf(-16.0f, eight[k][i * NG / J][c], s.o[k][2 * i + 1][c]);
+        s.o[k][2 * i][c] -= eight[k][i * NG / J][c & 1];
+        s.o[k][2 * i + 1][c] = fmaf(-16.0f, eight[k][i * NG / J][c & 1], s.o[k][2 * i + 1][c]);
       }
 }
 
 template <int D, int NG, int NT, int UN, int STAGES>
 struct AttnShape {
   static constexpr int ROWS = 8 * NT, UNIT = kv4_unit_bytes(D, D / NG), STAGE = UN * UNIT, RING = STAGES * STAGE;
-  static constexpr int PITCH = D + 4;  // of a row of partial o in shared memory
-  static constexpr int JOIN = AT_WARPS * ROWS * (PITCH + 2) * 4;
-  static constexpr int DATA = AT_WARPS * RING > JOIN ? AT_WARPS * RING : JOIN;
-  static constexpr int HEAD = 256;     // barriers, abort flag, sums
-  static constexpr int SMEM = HEAD + DATA;
+  static constexpr int HEAD = 256;           // barriers, abort flag
+  static constexpr int SMEM = HEAD + AT_WARPS * RING;
   static constexpr int PART = ROWS * (D + 2);  // floats of a part in the workspace: o, m, l
 };
 
 template <int D, int NG, int NT, int UN, int STAGES>
-__global__ void __launch_bounds__(AT_WARPS * 32) kv4_attn_kernel(AttnParams p) {
+__global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : 1) kv4_attn_kernel(AttnParams p) {
   using S = AttnShape<D, NG, NT, UN, STAGES>;
   constexpr int J = D / 32, ROWS = S::ROWS;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -349,277 +348,298 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attn_kernel(AttnParams p) {
   if (threadIdx.x < AT_WARPS * STAGES) mbar_init(bars + threadIdx.x, 1);
   if (threadIdx.x == 0) *abort_flag = 0;
   fence_mbar_init();
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
   const long long line = line_length<ROWS>(p);
-  __syncthreads();  // the barriers are set up
-  const long long piece = max((line + gridDim.x - 1) / gridDim.x, static_cast<long long>(AT_PIECE));
-  long long at = piece * blockIdx.x;
+  const long long piece = max((line + p.pieces - 1) / p.pieces, static_cast<long long>(AT_PIECE));
+  const int me = blockIdx.x * AT_WARPS + warp;  // this warp's piece
+  long long at = piece * me;
   const long long stop = min(at + piece, line);
-  if (threadIdx.x == 0) p.cuts[blockIdx.x].parts = 0;
+  if (lane == 0) p.cuts[me].parts = 0;
+  if (at >= stop) return;
   const WaitCtx ctx{abort_flag, p.status};
   const float cq = p.a.scale * LOG2E, cs = cq * Q4_LO_UNIT;
   const int page_units = 1 << (p.c.page_shift - 4);
+  uint32_t phase = 0;  // tiles this warp has taken from its ring so far
   int seq = 0;
   long long seq_at = 0;
-  uint32_t phase = 0;  // tiles this warp has taken from its ring so far
-  while (at < stop) {
-    // ---- the problem at `at`, and how much of it lies in this piece -------------------------------------------------------
-    if (!find_sequence<ROWS>(p, at, &seq, &seq_at)) break;
-    Problem pr;
-    pr.rows = kv4_rows(p.c, p.a.slots, p.a.ind, seq, p.a.T, p.status);
-    pr.units = seq_units(p, pr.rows, &pr.u_begin);
-    const int span = pr.units + AT_START;
-    const long long index = (at - seq_at) / span;
-    const int tiles = seq_problems<ROWS>(p, pr.rows) / p.c.heads;
-    pr.head = static_cast<int>(index / tiles);
-    pr.tile = static_cast<int>(index % tiles);
-    const long long start = seq_at + index * span;  // of the problem, on the line
-    const bool continued = at > start;
-    const int from = max(static_cast<int>(at - start) - AT_START, 0);
-    const int upto = max(static_cast<int>(min(static_cast<long long>(span), stop - start)) - AT_START, 0);
-    if (threadIdx.x == 0 && !continued && start + span > stop) {
-      // pieces [lo, hi] hold its units: this one does not if it ends among the empty places
-      const long long lo = (start + AT_START) / piece, hi = (start + span - 1) / piece;
-      Cut cut;
-      cut.parts = hi > lo ? static_cast<int>(hi - lo) + 1 : 0;
-      cut.first = static_cast<int>(lo * 2 + (lo == blockIdx.x ? 1 : 0));
-      cut.next = static_cast<int>(lo * 2 + 2);
-      cut.row_begin = pr.rows.begin;
-      cut.n_rows = (pr.rows.end - pr.rows.begin) * p.rep;
-      cut.head = pr.head;
-      cut.tile = pr.tile;
-      cut.unused = 0;
-      p.cuts[blockIdx.x] = cut;
-    }
-    at = min(start + span, stop);
-    if (from >= upto) continue;                     // the piece ends among the problem's empty places
-    const bool whole = from == 0 && upto == pr.units;
-    const int u0 = pr.u_begin + from, u1 = pr.u_begin + upto;
-    const int n_rows = (pr.rows.end - pr.rows.begin) * p.rep, first = pr.rows.length - (pr.rows.end - pr.rows.begin);
-    // ---- this warp's units, their pages, and the first tiles under way ------------------------------------------------------
-    const int end_row = min(pr.tile * ROWS + ROWS - 1, n_rows - 1);
-    const int visible = (max(first + end_row / p.rep + 1, 0) + KV4_UNIT - 1) / KV4_UNIT;  // units that hold a seen token
-    const int v1 = max(min(u1, visible), u0), len = v1 - u0;
-    const int w0 = u0 + static_cast<int>(static_cast<long long>(len) * warp / AT_WARPS);
-    const int w1 = u0 + static_cast<int>(static_cast<long long>(len) * (warp + 1) / AT_WARPS);
-    int page_base = w0, page_id = -1;  // lane i knows the page of unit page_base + i
-    auto look_up = [&](int base) {
-      page_base = base;
-      page_id = base + lane < w1 ? kv4_page(p.c, pr.rows.slot, (base + lane) * KV4_UNIT, p.status) : -1;
-    };
-    auto issue = [&](int u, uint32_t at_tile) {  // units [u, u + UN) into the tile's stage; returns which are there
-      if (u + UN > page_base + 32) look_up(u);
-      const int page = __shfl_sync(0xffffffffu, page_id, (u - page_base + lane) & 31);
-      const bool is = lane < UN && u + lane < w1 && page >= 0;
-      const uint32_t present = __ballot_sync(0xffffffffu, is);
-      const int st = at_tile % STAGES;
-      if (lane == 0) mbar_arrive_expect_tx(bar + st, __popc(present) * S::UNIT);
-      __syncwarp();
-      if (is)
-        bulk_load(ring + st * S::STAGE + lane * S::UNIT,
-                  p.c.pages + page * p.c.page_bytes +
-                      (static_cast<long long>(pr.head) * page_units + ((u + lane) & (page_units - 1))) * S::UNIT,
-                  S::UNIT, bar + st);
-      return present;
-    };
-    if (w0 < w1) look_up(w0);
-    const int n_tiles = (w1 - w0 + UN - 1) / UN;
-    uint32_t present = 0;  // UN bits a stage
-    for (int k = 0; k < STAGES && k < n_tiles; k++) present |= issue(w0 + k * UN, phase + k) << ((phase + k) % STAGES * UN);
-    // ---- queries ---------------------------------------------------------------------------------------------------------
-    Queries<D, NG, NT> q;
+  while (at < stop && find_sequence<ROWS>(p, at, &seq, &seq_at)) {
+    // ---- the sequence at `at`, and its problems from there on --------------------------------------------------------------
+    const Kv4Rows rows = kv4_rows(p.c, p.a.slots, p.a.ind, seq, p.a.T, p.status);
+    const int n_rows = (rows.end - rows.begin) * p.rep, first = rows.length - (rows.end - rows.begin);
+    int u_begin;
+    const int units = seq_units(p, rows, &u_begin), span = units + AT_START, problems = seq_problems<ROWS>(p, rows);
+    const int tiles = problems / p.c.heads;
+    for (int index = static_cast<int>((at - seq_at) / span); index < problems && at < stop; index++) {
+      const int head = index / tiles, row0 = (index - head * tiles) * ROWS;
+      const long long start = seq_at + static_cast<long long>(index) * span;  // of the problem, on the line
+      const bool continued = at > start;
+      const int from = max(static_cast<int>(at - start) - AT_START, 0);
+      const int upto = max(static_cast<int>(min(static_cast<long long>(span), stop - start)) - AT_START, 0);
+      if (lane == 0 && !continued && start + span > stop) {
+        // pieces [lo, hi] hold its units: this one does not if it ends among the empty places
+        const long long lo = (start + AT_START) / piece, hi = (start + span - 1) / piece;
+        Cut cut;
+        cut.parts = hi > lo ? static_cast<int>(hi - lo) + 1 : 0;
+        cut.first = static_cast<int>(lo * 2 + (lo == me ? 1 : 0));
+        cut.next = static_cast<int>(lo * 2 + 2);
+        cut.row_begin = rows.begin;
+        cut.n_rows = min(n_rows - row0, ROWS);
+        cut.head = head;
+        cut.row0 = row0;
+        cut.unused = 0;
+        p.cuts[me] = cut;
+      }
+      at = min(start + span, stop);
+      if (from >= upto) continue;  // the piece ends among the problem's empty places
+      // ---- its units in this piece, their pages, and the first tiles under way ----------------------------------------------
+      const int last_row = min(row0 + ROWS, n_rows) - 1;
+      const int visible = (max(first + last_row / p.rep + 1, 0) + KV4_UNIT - 1) / KV4_UNIT;  // units that hold a seen token
+      const int w0 = u_begin + from, w1 = min(u_begin + upto, visible);
+      int page_base = w0, page_id = -1;  // lane i knows the page of unit page_base + i
+      auto look_up = [&](int base) {
+        page_base = base;
+        page_id = base + lane < w1 ? kv4_page(p.c, rows.slot, (base + lane) * KV4_UNIT, p.status) : -1;
+      };
+      auto issue = [&](int u, uint32_t at_tile) {  // units [u, u + UN) into the tile's stage; returns which are there
+        if (u + UN > page_base + 32) look_up(u);
+        const int page = __shfl_sync(0xffffffffu, page_id, (u - page_base + lane) & 31);
+        const bool is = lane < UN && u + lane < w1 && page >= 0;
+        const uint32_t present = __ballot_sync(0xffffffffu, is);
+        const int st = at_tile % STAGES;
+        if (lane == 0) mbar_arrive_expect_tx(bar + st, __popc(present) * S::UNIT);
+        __syncwarp();
+        if (is)
+          bulk_load(ring + st * S::STAGE + lane * S::UNIT,
+                    p.c.pages + page * p.c.page_bytes +
+                        (static_cast<long long>(head) * page_units + ((u + lane) & (page_units - 1))) * S::UNIT,
+                    S::UNIT, bar + st);
+        return present;
+      };
+      const int n_tiles = w0 < w1 ? (w1 - w0 + UN - 1) / UN : 0;
+      if (n_tiles > 0) look_up(w0);
+      uint32_t present = 0;  // UN bits a stage
+      for (int k = 0; k < STAGES && k < n_tiles; k++) present |= issue(w0 + k * UN, phase + k) << ((phase + k) % STAGES * UN);
+      // ---- queries -------------------------------------------------------------------------------------------------------
+      Queries<D, NG, NT> q;
 #pragma unroll
-    for (int k = 0; k < NT; k++) {
-      const int row = min(pr.tile * ROWS + k * 8 + g, n_rows - 1);
-      const __half* qp = static_cast<const __half*>(p.a.Q) + (pr.rows.begin + row / p.rep) * p.a.ldq +
-                         (pr.head * p.rep + row % p.rep) * D;
-      float sum[NG] = {};
+      for (int k = 0; k < NT; k++) {
+        const int row = min(row0 + k * 8 + g, n_rows - 1), token = row / p.rep;
+        const __half* qp = static_cast<const __half*>(p.a.Q) + (rows.begin + token) * p.a.ldq +
+                           (head * p.rep + row - token * p.rep) * D;
+        float sum[NG] = {};
 #pragma unroll
-      for (int j = 0; j < J; j++) {
-        const uint4 v = *reinterpret_cast<const uint4*>(qp + (4 * j + t) * 8);
-        // dims 0..7 of the word pair up as (0, 4), (2, 6) for the low nibbles' step and (1, 5), (3, 7) for the high ones'
-        q.b[k][2 * j][0] = __byte_perm(v.x, v.z, 0x5410);
-        q.b[k][2 * j][1] = __byte_perm(v.y, v.w, 0x5410);
-        q.b[k][2 * j + 1][0] = __byte_perm(v.x, v.z, 0x7632);
-        q.b[k][2 * j + 1][1] = __byte_perm(v.y, v.w, 0x7632);
-        const __half2* h = reinterpret_cast<const __half2*>(&v);
+        for (int j = 0; j < J; j++) {
+          const uint4 v = *reinterpret_cast<const uint4*>(qp + (4 * j + t) * 8);
+          // dims 0..7 of the word pair up as (0, 4), (2, 6) for the low nibbles' step and (1, 5), (3, 7) for the high ones'
+          q.b[k][2 * j][0] = __byte_perm(v.x, v.z, 0x5410);
+          q.b[k][2 * j][1] = __byte_perm(v.y, v.w, 0x5410);
+          q.b[k][2 * j + 1][0] = __byte_perm(v.x, v.z, 0x7632);
+          q.b[k][2 * j + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+          const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 f = __half22float2(h[i]);
-          sum[j * NG / J] += f.x + f.y;
+          for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(h[i]);
+            sum[j * NG / J] += f.x + f.y;
+          }
+        }
+#pragma unroll
+        for (int grp = 0; grp < NG; grp++) {
+          sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 1);
+          sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 2);
+          q.sum[2 * k][grp] = __shfl_sync(0xffffffffu, sum[grp], 8 * t) * cq;
+          q.sum[2 * k + 1][grp] = __shfl_sync(0xffffffffu, sum[grp], 8 * t + 4) * cq;
         }
       }
 #pragma unroll
-      for (int grp = 0; grp < NG; grp++) {
-        sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 1);
-        sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 2);
-        q.sum[2 * k][grp] = __shfl_sync(0xffffffffu, sum[grp], 8 * t) * cq;
-        q.sum[2 * k + 1][grp] = __shfl_sync(0xffffffffu, sum[grp], 8 * t + 4) * cq;
+      for (int r = 0; r < 2 * NT; r++) {  // rows behind the last repeat it
+        const int pos = first + min(row0 + (r >> 1) * 8 + 2 * t + (r & 1), n_rows - 1) / p.rep;
+        q.hi[r] = pos + 1;
+        q.lo[r] = p.a.window > 0 ? max(pos + 1 - p.a.window, 0) : 0;
       }
-    }
+      // every row sees tokens [all_lo, all_hi)
+      const int all_hi = first + row0 / p.rep + 1;
+      const int all_lo = p.a.window > 0 ? max(first + last_row / p.rep + 1 - p.a.window, 0) : 0;
+      RowState<D, NG, NT> s;
 #pragma unroll
-    for (int r = 0; r < 2 * NT; r++) {  // rows behind the last repeat it
-      const int pos = first + min(pr.tile * ROWS + (r >> 1) * 8 + 2 * t + (r & 1), n_rows - 1) / p.rep;
-      q.hi[r] = pos + 1;
-      q.lo[r] = p.a.window > 0 ? max(pos + 1 - p.a.window, 0) : 0;
-    }
-    // every row sees tokens [all_lo, all_hi)
-    const int all_hi = first + pr.tile * ROWS / p.rep + 1;
-    const int all_lo = p.a.window > 0 ? max(first + end_row / p.rep + 1 - p.a.window, 0) : 0;
-    RowState<D, NG, NT> s;
+      for (int r = 0; r < 2 * NT; r++) {
+        s.m[r] = -INFINITY;
+        s.l[r] = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 2 * NT; r++) {
-      s.m[r] = -INFINITY;
-      s.l[r] = 0.0f;
+        for (int grp = 0; grp < NG; grp++) s.z[r][grp] = 0.0f;
+      }
 #pragma unroll
-      for (int grp = 0; grp < NG; grp++) s.z[r][grp] = 0.0f;
-    }
+      for (int k = 0; k < NT; k++)
 #pragma unroll
-    for (int k = 0; k < NT; k++)
+        for (int i = 0; i < D / 16; i++)
 #pragma unroll
-      for (int i = 0; i < D / 16; i++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) s.o[k][i][c] = 0.0f;
-    s.e = -14;
-    // ---- tokens ------------------------------------------------------------------------------------------------------------
+          for (int c = 0; c < 4; c++) s.o[k][i][c] = 0.0f;
+      s.e = -14;
+      // ---- tokens ----------------------------------------------------------------------------------------------------------
 #pragma unroll 1
-    for (int i = 0; i < n_tiles; i++) {
-      const uint32_t n = phase + i, st = n % STAGES, here = (present >> (st * UN)) & ((1u << UN) - 1);
-      if (!mbar_wait_warp(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx)) continue;  // recorded; nothing hangs
-      const int tok0 = (w0 + i * UN) * KV4_UNIT;
-      const uint8_t* stage = ring + st * S::STAGE;
-      if (tok0 >= all_lo && tok0 + UN * KV4_UNIT <= all_hi && here == (1u << UN) - 1)
-        kv4_tile<D, NG, NT, UN, false>(stage, tok0, here, cs, q, s);
-      else
-        kv4_tile<D, NG, NT, UN, true>(stage, tok0, here, cs, q, s);
-      __syncwarp();
-      if (i + STAGES < n_tiles) {
-        present &= ~(((1u << UN) - 1) << (st * UN));
-        present |= issue(w0 + (i + STAGES) * UN, n + STAGES) << (st * UN);
+      for (int i = 0; i < n_tiles; i++) {
+        const uint32_t n = phase + i, st = n % STAGES, here = (present >> (st * UN)) & ((1u << UN) - 1);
+        if (!mbar_wait_warp(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx)) continue;  // recorded; nothing hangs
+        const int tok0 = (w0 + i * UN) * KV4_UNIT;
+        const uint8_t* stage = ring + st * S::STAGE;
+        if (tok0 >= all_lo && tok0 + UN * KV4_UNIT <= all_hi && here == (1u << UN) - 1)
+          kv4_tile<D, NG, NT, UN, false>(stage, tok0, here, cs, q, s);
+        else
+          kv4_tile<D, NG, NT, UN, true>(stage, tok0, here, cs, q, s);
+        __syncwarp();
+        if (i + STAGES < n_tiles) {
+          present &= ~(((1u << UN) - 1) << (st * UN));
+          present |= issue(w0 + (i + STAGES) * UN, n + STAGES) << (st * UN);
+        }
       }
-    }
-    phase += n_tiles;
-    // ---- join the warps -----------------------------------------------------------------------------------------------------
-    float* so = reinterpret_cast<float*>(smem + S::HEAD);               // [AT_WARPS][ROWS][PITCH], m and l behind a row's o
-    __syncthreads();                                                    // every ring is drained
-#pragma unroll
-    for (int r = 0; r < 2 * NT; r++) {
-      const int row = (r >> 1) * 8 + 2 * t + (r & 1);
-      float* mine = so + (warp * ROWS + row) * (S::PITCH + 2);
-      s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 4);
-      s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 8);
-      s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 16);
+      phase += n_tiles;
+      // ---- rows 2t, 2t + 1: finish, or leave a part ---------------------------------------------------------------------------
+      const bool whole = from == 0 && upto == units;
+      float* part = p.part + (static_cast<long long>(me) * 2 + (continued ? 0 : 1)) * S::PART;
       const float down = pow2i(s.e - 14);
 #pragma unroll
-      for (int grp = 0; grp < NG; grp++) {
-        s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 4);
-        s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 8);
-        s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 16);
-      }
+      for (int r = 0; r < 2 * NT; r++) {
+        const int in_tile = (r >> 1) * 8 + 2 * t + (r & 1), row = row0 + in_tile;
+        s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 4);
+        s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 8);
+        s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 16);
 #pragma unroll
-      for (int i = 0; i < J; i++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const float zero = s.z[r][i * NG / J];
-          mine[32 * i + 4 * g + 2 * k] = fmaf(s.o[r >> 1][2 * i][2 * k + (r & 1)] * Q4_LO_UNIT, down, zero);
-          mine[32 * i + 4 * g + 2 * k + 1] = fmaf(s.o[r >> 1][2 * i + 1][2 * k + (r & 1)] * Q4_HI_UNIT, down, zero);
+        for (int grp = 0; grp < NG; grp++) {
+          s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 4);
+          s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 8);
+          s.z[r][grp] += __shfl_xor_sync(0xffffffffu, s.z[r][grp], 16);
         }
-      if (g == 0) {
-        mine[S::PITCH] = s.m[r];
-        mine[S::PITCH + 1] = s.l[r];
-      }
-    }
-    __syncthreads();
-    float* part = p.part + (static_cast<long long>(blockIdx.x) * 2 + (continued ? 0 : 1)) * S::PART;
-    for (int i = threadIdx.x; i < ROWS * D; i += AT_WARPS * 32) {
-      const int r = i / D, d = i % D, row = pr.tile * ROWS + r;
-      if (row >= n_rows) break;
-      const float* one = so + r * (S::PITCH + 2);
-      constexpr int STEP = ROWS * (S::PITCH + 2);
-      float m = one[S::PITCH];
+        if (row >= n_rows) continue;
+        const int token = row / p.rep, h = head * p.rep + row - token * p.rep;
+        const long long out = rows.begin + token;
+        const float inv = s.l[r] == 0.0f ? 0.0f : 1.0f / s.l[r];  // (a row that saw nothing has only zeros)
 #pragma unroll
-      for (int w = 1; w < AT_WARPS; w++) m = fmaxf(m, one[w * STEP + S::PITCH]);
-      float l = 0.0f, o = 0.0f;
+        for (int i = 0; i < J; i++) {
+          float v[4];
 #pragma unroll
-      for (int w = 0; w < AT_WARPS; w++) {
-        const float mw = one[w * STEP + S::PITCH], lw = one[w * STEP + S::PITCH + 1];
-        if (lw == 0.0f) continue;  // saw nothing (a NaN sum is kept)
-        const float f = exp2_approx(mw - m);
-        l = fmaf(lw, f, l);
-        o = fmaf(one[w * STEP + d], f, o);
-      }
-      if (whole) {
-        const long long out = pr.rows.begin + row / p.rep;
-        const int h = pr.head * p.rep + row % p.rep;
-        static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
-        if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
-      } else {
-        part[i] = o;
-        if (d == 0) {
-          part[ROWS * D + r] = m;
-          part[ROWS * D + ROWS + r] = l;
+          for (int k = 0; k < 2; k++) {
+            const float zero = s.z[r][i * NG / J];
+            v[2 * k] = fmaf(s.o[r >> 1][2 * i][2 * k + (r & 1)] * Q4_LO_UNIT, down, zero);
+            v[2 * k + 1] = fmaf(s.o[r >> 1][2 * i + 1][2 * k + (r & 1)] * Q4_HI_UNIT, down, zero);
+          }
+          if (whole)
+            *reinterpret_cast<uint2*>(static_cast<__half*>(p.a.O) + out * p.a.ldo + h * D + 32 * i + 4 * g) =
+                make_uint2(pack_half2(v[0] * inv, v[1] * inv), pack_half2(v[2] * inv, v[3] * inv));
+          else
+            *reinterpret_cast<float4*>(part + in_tile * D + 32 * i + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        if (g == 0) {
+          if (!whole) {
+            part[ROWS * D + in_tile] = s.m[r];
+            part[ROWS * D + ROWS + in_tile] = s.l[r];
+          } else if (p.a.lse) {
+            p.a.lse[out * p.a.ldl + h] = s.l[r] == 0.0f ? -INFINITY : fmaf(s.m[r], LN2, logf(s.l[r]));
+          }
         }
       }
     }
-    fence_proxy_async_smem();  // the next tiles' copies come after what was read and written here
-    __syncthreads();
   }
 }
 
 constexpr int JOIN_THREADS = 256;
 
-// Joins the parts of problems that were cut: CTA (c, r) takes row r of the problem that piece c left to be joined.
+// Joins the parts of problems that were cut.  An item is every `split`-th row of one problem; CTA b looks at items b,
+// b + gridDim.x, ... all at once, for most pieces end without a cut, and joins those that there are.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p) {
-  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, CHUNK = 256;
+__global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, int split) {
+  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, CHUNK = 256, FEW = 8;
   __shared__ float weight[CHUNK], top[JOIN_THREADS / 32], so[GROUPS][D], sl[JOIN_THREADS / 32];
-  pdl_wait();
-  const Cut cut = p.cuts[blockIdx.x];
-  const int r = blockIdx.y, row = cut.tile * ROWS + r, n = cut.parts;
-  if (n == 0 || row >= cut.n_rows) return;
-  auto part_of = [&](int i) { return p.part + static_cast<long long>(i == 0 ? cut.first : cut.next + 2 * (i - 1)) * PART; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x % D, group = threadIdx.x / D;
-  // the largest maximum, then every part's weight
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += JOIN_THREADS) m = fmaxf(m, part_of(i)[ROWS * D + r]);
-#pragma unroll
-  for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  if (lane == 0) top[warp] = m;
+  __shared__ int list[JOIN_THREADS], listed;
+  if (threadIdx.x == 0) listed = 0;
   __syncthreads();
-  for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, top[w]);
-  float l = 0.0f, o = 0.0f;
-  for (int i0 = 0; i0 < n; i0 += CHUNK) {
-    const int i = i0 + threadIdx.x;
-    if (i < n) {
-      const float* part = part_of(i);
-      const float mi = part[ROWS * D + r], li = part[ROWS * D + ROWS + r];
-      const float f = li == 0.0f ? 0.0f : exp2_approx(mi - m);  // (a part that saw nothing holds no numbers)
-      weight[threadIdx.x] = f;
-      if (li != 0.0f) l = fmaf(li, f, l);
+  pdl_wait();
+  {
+    // (the launch sees to it that a CTA has at most JOIN_THREADS items)
+    const int item = blockIdx.x + threadIdx.x * gridDim.x;
+    if (item < p.pieces * split) {
+      const Cut& c = p.cuts[item / split];
+      if (c.parts > 0 && item % split < c.n_rows) list[atomicAdd(&listed, 1)] = item;
     }
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x % D, group = threadIdx.x / D;
+  for (int at = 0; at < listed; at++) {
+    const Cut cut = p.cuts[list[at] / split];
+    const int n = cut.parts, row_begin = list[at] % split, row_step = split;
+    auto part_of = [&](int i) { return p.part + static_cast<long long>(i == 0 ? cut.first : cut.next + 2 * (i - 1)) * PART; };
+  auto write = [&](int r, int d, float m, float l, float o) {
+    const int row = cut.row0 + r, token = row / p.rep, h = cut.head * p.rep + row - token * p.rep;
+    const long long out = cut.row_begin + token;
+    static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
+    if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
+  };
+  if (n <= FEW) {  // every thread on its own
+    for (int r = row_begin + group * row_step; r < cut.n_rows; r += row_step * GROUPS) {
+      float mi[FEW], li[FEW], v[FEW], m = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll
+      for (int i = 0; i < FEW; i++) {
+        mi[i] = -INFINITY;
+        li[i] = v[i] = 0.0f;
+        if (i < n) {
+          const float* part = part_of(i);
+          mi[i] = part[ROWS * D + r];
+          li[i] = part[ROWS * D + ROWS + r];
+          v[i] = part[r * D + d];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < FEW; i++) m = fmaxf(m, mi[i]);
+#pragma unroll
+      for (int i = 0; i < FEW; i++) {
+        if (li[i] == 0.0f) continue;
+        const float f = exp2_approx(mi[i] - m);
+        l = fmaf(li[i], f, l);
+        o = fmaf(v[i], f, o);
+      }
+      write(r, d, m, l, o);
+    }
+    continue;
+  }
+  for (int r = row_begin; r < cut.n_rows; r += row_step) {
+    // the largest maximum, then every part's weight
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += JOIN_THREADS) m = fmaxf(m, part_of(i)[ROWS * D + r]);
+#pragma unroll
+    for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    if (lane == 0) top[warp] = m;
     __syncthreads();
-    const int end = min(n - i0, CHUNK);
+    for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, top[w]);
+    float l = 0.0f, o = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += CHUNK) {
+      const int i = i0 + threadIdx.x;
+      if (i < n) {
+        const float* part = part_of(i);
+        const float mi = part[ROWS * D + r], li = part[ROWS * D + ROWS + r];
+        const float f = li == 0.0f ? 0.0f : exp2_approx(mi - m);  // (the weight of a part that saw nothing)
+        weight[threadIdx.x] = f;
+        if (li != 0.0f) l = fmaf(li, f, l);
+      }
+      __syncthreads();
+      const int end = min(n - i0, CHUNK);
 #pragma unroll 8
-    for (int k = group; k < end; k += GROUPS) {
-      const float f = weight[k], v = part_of(i0 + k)[r * D + d];
-      o = f == 0.0f ? o : fmaf(v, f, o);
+      for (int k = group; k < end; k += GROUPS) o = fmaf(part_of(i0 + k)[r * D + d], weight[k], o);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k /= 2) l += __shfl_xor_sync(0xffffffffu, l, k);
+    if (lane == 0) sl[warp] = l;
+    so[group][d] = o;
+    __syncthreads();
+    if (group == 0) {
+      l = o = 0.0f;
+      for (int w = 0; w < JOIN_THREADS / 32; w++) l += sl[w];
+      for (int k = 0; k < GROUPS; k++) o += so[k][d];
+      write(r, d, m, l, o);
     }
     __syncthreads();
   }
-#pragma unroll
-  for (int k = 16; k > 0; k /= 2) l += __shfl_xor_sync(0xffffffffu, l, k);
-  if (lane == 0) sl[warp] = l;
-  so[group][d] = o;
-  __syncthreads();
-  if (group != 0) return;
-  l = o = 0.0f;
-  for (int w = 0; w < JOIN_THREADS / 32; w++) l += sl[w];
-  for (int k = 0; k < GROUPS; k++) o += so[k][d];
-  const long long out = cut.row_begin + row / p.rep;
-  const int h = cut.head * p.rep + row % p.rep;
-  static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
-  if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
+  }
 }
 
 constexpr int AT_MOST_PER_SM = 4;
@@ -646,16 +666,24 @@ cudaError_t per_sm_of(int* per_sm) {
 template <int D, int NG, int NT, int UN, int STAGES>
 cudaError_t launch_attn(AttnParams& p, int most_rows, int sm_count, cudaStream_t stream) {
   using S = AttnShape<D, NG, NT, UN, STAGES>;
-  auto kernel = kv4_attn_kernel<D, NG, NT, UN, STAGES>;
   int per_sm = 0;
   cudaError_t e = per_sm_of<D, NG, NT, UN, STAGES>(&per_sm);
   if (e != cudaSuccess) return e;
-  p.pieces = sm_count * per_sm;
-  e = launch_with_pdl(kernel, dim3(p.pieces), dim3(AT_WARPS * 32), S::SMEM, stream, p);
+  // no more warps than pieces of the smallest size, if the tables are narrow
+  const long long most = (static_cast<long long>(p.c.table_width) << (p.c.page_shift - 4)) + AT_START;
+  const long long problems = static_cast<long long>(p.c.heads) *
+                             (p.a.ind ? static_cast<long long>(p.a.T) * p.rep / S::ROWS + p.a.n
+                                      : static_cast<long long>(p.a.n) * ((p.rep + S::ROWS - 1) / S::ROWS));
+  int ctas = sm_count * per_sm;
+  if (problems < ctas * AT_WARPS) ctas = static_cast<int>(min(static_cast<long long>(ctas), (problems * most + AT_PIECE * AT_WARPS - 1) / (AT_PIECE * AT_WARPS)));
+  p.pieces = ctas * AT_WARPS;
+  e = launch_with_pdl(kv4_attn_kernel<D, NG, NT, UN, STAGES>, dim3(ctas), dim3(AT_WARPS * 32), S::SMEM, stream, p);
   if (e != cudaSuccess) return e;
-  if (p.pieces == 1) return cudaSuccess;
-  const dim3 cuts(p.pieces - 1, min(most_rows, S::ROWS));
-  return launch_with_pdl(kv4_join_kernel<D, S::ROWS>, cuts, dim3(JOIN_THREADS), 0, stream, p);
+  // few problems leave many parts each: an item a row; many leave few: an item as many rows as a CTA joins at a time
+  const int rows = min(most_rows, S::ROWS), split = problems <= sm_count ? rows : (rows + JOIN_THREADS / D - 1) / (JOIN_THREADS / D);
+  const int join_ctas = min(p.pieces * split, 4 * sm_count);
+  static_assert(AT_MOST_PER_SM * AT_WARPS * S::ROWS <= 4 * JOIN_THREADS, "a CTA's items of the joining kernel");
+  return launch_with_pdl(kv4_join_kernel<D, S::ROWS>, dim3(join_ctas), dim3(JOIN_THREADS), 0, stream, p, split);
 }
 
 template <int D, int NG>
@@ -669,13 +697,13 @@ int row_tiles(const Kv4View& c, int T, int n, int q_heads, bool one_each) { retu
 }  // namespace
 
 size_t kv4_attention_workspace(const Kv4View& c, int T, int n, int q_heads, int sm_count) {
-  return static_cast<size_t>(sm_count) * AT_MOST_PER_SM * (sizeof(Cut) + 2 * (16 * (c.D + 2)) * sizeof(float));
+  return static_cast<size_t>(sm_count) * AT_MOST_PER_SM * AT_WARPS * (sizeof(Cut) + 2 * (16 * (c.D + 2)) * sizeof(float));
 }
 
 int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, size_t workspace_bytes, int sm_count,
                          uint32_t* status, cudaStream_t stream, const char** err) {
   Cut* cuts = static_cast<Cut*>(workspace);
-  AttnParams p{c, a, a.q_heads / c.heads, 0, cuts, reinterpret_cast<float*>(cuts + sm_count * AT_MOST_PER_SM), status};
+  AttnParams p{c, a, a.q_heads / c.heads, 0, cuts, reinterpret_cast<float*>(cuts + sm_count * AT_MOST_PER_SM * AT_WARPS), status};
   const int nt = row_tiles(c, a.T, a.n, a.q_heads, a.ind == nullptr);
   const int most_rows = a.ind ? 8 * nt : p.rep;  // rows of a problem that can be there
   const int ng = c.D / c.G;

@@ -318,7 +318,10 @@ def test_bad_slots_and_pages_are_not_followed(ph, dev):
     lens = [60, 50, 40]
     s = Setup(ph, dev, lens, 2, 64, 64, 16)
     q = torch.randn(3, 4 * 64, device=dev).half()
-    want, _ = attend(s, q, [0, 1, 2, 3], 0.125)
+    # (where sequences are cut depends on the batch, so a batch with another length in it agrees to rounding)
+    want, _, tol, _ = reference(s, q, [0, 1, 2, 3], 2, 0.125, 0)
+    near = lambda o, rows: bool(((o[rows].double() - want[rows]).abs() <= tol[rows]).all())  # noqa: E731
+    assert near(attend(s, q, [0, 1, 2, 3], 0.125)[0], [0, 1, 2])
     assert ph.device_status() == 0
     for bad in (-1, 5, 2 ** 31 - 1):
         slots = s.slots.clone()
@@ -327,7 +330,7 @@ def test_bad_slots_and_pages_are_not_followed(ph, dev):
         with pytest.raises(ph.PhobosError) as e:
             ph.device_status()
         assert e.value.code == ph.PH_ERR_INVALID
-        assert torch.equal(o[[0, 2]], want[[0, 2]]) and bool((o[1] == 0).all()) and bool(torch.isinf(lse[1]).all())
+        assert near(o, [0, 2]) and bool((o[1] == 0).all()) and bool(torch.isinf(lse[1]).all())
         assert ph.device_status() == 0
     pages = s.cache.pages.clone()
     for bad in (-1, s.cache.refs.numel(), 2 ** 31 - 1):
@@ -336,7 +339,7 @@ def test_bad_slots_and_pages_are_not_followed(ph, dev):
         o, _ = attend(s, q, [0, 1, 2, 3], 0.125)
         with pytest.raises(ph.PhobosError):
             ph.device_status()
-        assert torch.equal(o[1:], want[1:]) and bool(torch.isfinite(o[0]).all())
+        assert near(o, [1, 2]) and bool(torch.isfinite(o[0]).all())
         keep = torch.tensor([0, 40], dtype=torch.int32, device=dev)
         kv = torch.randn(40, 128, device=dev).half()
         ph.kv4_append(s.cache, 0, kv, kv, s.slots[:1], keep)       # tokens 20..59: the ones of the bad page are left out
@@ -354,7 +357,7 @@ def test_bad_slots_and_pages_are_not_followed(ph, dev):
     o, _ = attend(s, q, [0, 1, 2, 3], 0.125, window=64)
     with pytest.raises(ph.PhobosError):
         ph.device_status()
-    assert torch.equal(o[:2], attend(s, q, [0, 1, 2, 3], 0.125, window=64)[0][:2]) if False else True
+    assert near(o, [0, 1])
     s.cache.lens.copy_(long)
     # an indptr that does not ascend or leaves the rows: nothing outside is touched
     o = torch.full((6, 256), 7.0, device=dev).half()
