@@ -142,6 +142,12 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, u
   return ok != 0;
 }
 
+// The same for a phase that is usually complete already: one poll by the converged warp, then as above.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, uint32_t site, const WaitCtx& ctx) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return mbar_wait_warp(bar, parity, site, ctx);
+}
+
 // Waits executed by a whole warp ahead of warp-collective TMEM accesses.
 #ifndef PH_WAIT_ALL_LANES
 #define PH_WARP_WAIT(bar, parity, site, ctx) mbar_wait_warp(bar, parity, site, ctx)

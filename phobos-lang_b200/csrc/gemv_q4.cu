@@ -10,10 +10,12 @@
 // byte order 0, 2, 1, 3: the A operand of one matrix step from one word.
 // The kernel: a CTA of eight multiplying warps and one that copies.  The multiplying warps form WR x WK: WR along the rows
 // of W (RT tiles of 16 each), WK along the columns (a block of 128 each).  A stage of the ring holds WR RT x WK blocks and
-// the WK * 128 columns of up to 8 NT rows of X, brought by bulk copies; X rows stand 64 bytes off a multiple of 128
-// apart, so that a lane's 16-byte reads (the B operand of two matrix steps) meet no bank twice.  CTAs stay: each takes
-// row groups in turn, and the copying warp runs ahead into the next group while the last one is written.
+// WK * 128 columns of up to eight rows of X, brought by bulk copies; X rows stand 64 bytes off a multiple of 128 apart, so
+// that a lane's 16-byte reads (the B operand of two matrix steps) meet no bank twice.  The tiles of W are dealt out evenly
+// over a grid that fills the GPU: a CTA whose share is not a multiple of WR RT leaves some products idle, which costs
+// nothing as long as the bytes are what is waited for.
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -23,6 +25,7 @@ namespace ph {
 namespace {
 
 constexpr int GV_WARPS = 8;                            // multiplying warps
+constexpr int GV_PER_SM = 2;                            // CTAs that share an SM
 constexpr int GV_THREADS = (GV_WARPS + 1) * 32;
 constexpr uint32_t ONES = 0x3c003c00u;                 // two f16 ones
 enum : uint32_t { SITE_GEMV_FULL = 0x42, SITE_GEMV_EMPTY = 0x43 };
@@ -32,26 +35,22 @@ struct GemvParams {
   const uint8_t* W;
   void* Y;
   long long ldx, ldy;
-  int M, N, K, G, block_bytes, kblocks, tiles;         // tiles of 16 rows
-  int row_groups, m_groups;
+  int M, N, K, kblocks, tiles;         // tiles of 16 rows
+  int stages, stage_bytes;
   float alpha, beta;
   int out_f32;
   uint32_t* status;
 };
 
-template <int NT, int RT, int WR>
+template <int RT, int WR, int GS>
 struct GemvShape {
-  static constexpr int WK = GV_WARPS / WR, TILES = RT * WR, ROWS = 16 * TILES, COLS = 8 * NT;
-  static constexpr int X_PITCH = WK * 256 + 64, X_BYTES = COLS * X_PITCH;
-  static constexpr int W_MOST = TILES * WK * (1024 + 256);  // (at G = 32)
-  static constexpr int STAGE = (X_BYTES + W_MOST + 127) / 128 * 128;
-  static constexpr int OUT_PITCH = ROWS + 4, OUT = WK * COLS * OUT_PITCH * 4;
-  static constexpr int HEAD = 256;
-  static constexpr int TWO = (226 * 1024 / 2 - 1024 - HEAD - OUT) / STAGE;  // stages with two CTAs on an SM
-  static constexpr int ROOM = TWO >= 2 ? TWO : (226 * 1024 - HEAD - OUT) / STAGE;
-  static constexpr int STAGES = ROOM > 6 ? 6 : ROOM;
-  static constexpr int SMEM = HEAD + STAGES * STAGE + OUT;
-  static_assert(STAGES >= 2 && SMEM <= 227 * 1024, "stages of the ring");
+  static constexpr int WK = GV_WARPS / WR, TILES = RT * WR, ROWS = 16 * TILES;
+  static constexpr int X_PITCH = WK * 256 + 64;
+  static constexpr int BLOCK = 1024 + 64 * (8 / GS);   // GS matrix steps of 16 columns are a group
+  static constexpr int W_BYTES = TILES * WK * BLOCK;
+  static constexpr int OUT_PITCH = ROWS + 4, OUT = WK * 8 * OUT_PITCH * 4;
+  static constexpr int HEAD = 256, MOST_STAGES = 8;
+  static_assert(X_PITCH % 128 == 64 && W_BYTES % 64 == 0, "shared memory layout");
 };
 
 __device__ __forceinline__ void gemv_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -60,17 +59,19 @@ __device__ __forceinline__ void gemv_bulk_load(void* dst, const void* src, uint3
                : "memory");
 }
 
-template <int NT, int RT, int WR>
-__global__ void __launch_bounds__(GV_THREADS) gemv_q4_kernel(GemvParams p) {
-  using S = GemvShape<NT, RT, WR>;
+// CTA (x, y): its share of the tiles of W, rows 8y .. 8y + 7 of X.
+template <int RT, int WR, int GS>
+__global__ void __launch_bounds__(GV_THREADS, GV_PER_SM) gemv_q4_kernel(GemvParams p) {
+  using S = GemvShape<RT, WR, GS>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
-  uint64_t* empty = full + S::STAGES;
+  uint64_t* empty = full + S::MOST_STAGES;
   uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + 192);
-  uint8_t* ring = smem + S::HEAD;
-  float* out = reinterpret_cast<float*>(ring + S::STAGES * S::STAGE);
+  static_assert(16 * S::MOST_STAGES <= 192, "shared memory head");
+  float* out = reinterpret_cast<float*>(smem + S::HEAD);
+  uint8_t* ring = smem + S::HEAD + S::OUT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (threadIdx.x < S::STAGES) {
+  if (threadIdx.x < p.stages) {
     mbar_init(full + threadIdx.x, 1);
     mbar_init(empty + threadIdx.x, GV_WARPS);
   }
@@ -80,129 +81,133 @@ __global__ void __launch_bounds__(GV_THREADS) gemv_q4_kernel(GemvParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const WaitCtx ctx{abort_flag, p.status};
-  const int chunks = (p.kblocks + S::WK - 1) / S::WK, groups = p.row_groups * p.m_groups;
-  uint32_t it = 0;
+  const int chunks = (p.kblocks + S::WK - 1) / S::WK;
+  const int first = static_cast<int>(static_cast<long long>(p.tiles) * blockIdx.x / gridDim.x);
+  const int last = static_cast<int>(static_cast<long long>(p.tiles) * (blockIdx.x + 1) / gridDim.x);
+  const int m0 = blockIdx.y * 8, n_m = min(8, p.M - m0);
+  const int x_bytes = n_m * S::X_PITCH;  // of a stage
+  int st = 0;
+  uint32_t parity = 0;
   if (warp == GV_WARPS) {
     // ---- copies ---------------------------------------------------------------------------------------------------------
-    for (int grp = blockIdx.x; grp < groups; grp += gridDim.x) {
-      // neighbours take the same rows of W for other rows of X: W comes from HBM once
-      const int tile0 = grp / p.m_groups * S::TILES, m0 = grp % p.m_groups * S::COLS;
-      const int n_tiles = min(S::TILES, p.tiles - tile0), n_m = min(S::COLS, p.M - m0);
-      for (int c = 0; c < chunks; c++, it++) {
-        const int st = it % S::STAGES, kb = c * S::WK;
-        if (it >= S::STAGES && !mbar_wait_warp(empty + st, (it / S::STAGES - 1) & 1, SITE_GEMV_EMPTY, ctx)) return;
-        const int n_kb = min(S::WK, p.kblocks - kb);
-        const uint32_t w_bytes = n_kb * p.block_bytes, x_bytes = min(n_kb * 128, p.K - kb * 128) * 2;
-        uint8_t* stage = ring + st * S::STAGE;
-        if (lane == 0) mbar_arrive_expect_tx(full + st, n_tiles * w_bytes + n_m * x_bytes);
+    bool refill = false;
+    for (int tile0 = first; tile0 < last; tile0 += S::TILES) {
+      const int n_tiles = min(S::TILES, last - tile0);
+      for (int c = 0; c < chunks; c++) {
+        const int kb = c * S::WK, n_kb = min(S::WK, p.kblocks - kb);
+        if (refill && !mbar_wait_warp(empty + st, parity ^ 1, SITE_GEMV_EMPTY, ctx)) return;
+        const uint32_t w_each = n_kb * S::BLOCK, x_each = min(n_kb * 128, p.K - kb * 128) * 2;
+        uint8_t* stage = ring + st * p.stage_bytes;
+        if (lane == 0) mbar_arrive_expect_tx(full + st, n_tiles * w_each + n_m * x_each);
         __syncwarp();
-        for (int i = lane; i < n_tiles + n_m; i += 32) {
-          if (i < n_tiles)
-            gemv_bulk_load(stage + S::X_BYTES + i * S::WK * p.block_bytes,
-                           p.W + (static_cast<long long>(tile0 + i) * p.kblocks + kb) * p.block_bytes, w_bytes, full + st);
-          else
-            gemv_bulk_load(stage + (i - n_tiles) * S::X_PITCH, p.X + (m0 + i - n_tiles) * p.ldx + kb * 128, x_bytes, full + st);
+        if (lane < n_tiles)
+          gemv_bulk_load(stage + x_bytes + lane * S::WK * S::BLOCK, p.W + (static_cast<long long>(tile0 + lane) * p.kblocks + kb) * S::BLOCK,
+                         w_each, full + st);
+        else if (lane - n_tiles < n_m)
+          gemv_bulk_load(stage + (lane - n_tiles) * S::X_PITCH, p.X + (m0 + lane - n_tiles) * p.ldx + kb * 128, x_each, full + st);
+        if (++st == p.stages) {
+          st = 0;
+          parity ^= 1;
+          refill = true;
         }
       }
     }
     return;
   }
   // ---- products -----------------------------------------------------------------------------------------------------------
+  static_assert(S::TILES + 8 <= 32, "a lane for every copy");
   const int wr = warp / S::WK, wk = warp % S::WK;
-  const int steps_per_group = p.G / 16;
-  for (int grp = blockIdx.x; grp < groups; grp += gridDim.x) {
-    const int tile0 = grp / p.m_groups * S::TILES, m0 = grp % p.m_groups * S::COLS;
-    float y[RT][NT][4];
+  const int x_row = min(g, n_m - 1) * S::X_PITCH;  // columns of the product behind the last row repeat it
+  for (int tile0 = first; tile0 < last; tile0 += S::TILES) {
+    float y[RT][4];
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) y[r][n][i] = 0.0f;
+      for (int i = 0; i < 4; i++) y[r][i] = 0.0f;
 #pragma unroll 1
-    for (int c = 0; c < chunks; c++, it++) {
-      const int st = it % S::STAGES, kb = c * S::WK + wk;
-      const bool ok = mbar_wait_warp(full + st, (it / S::STAGES) & 1, SITE_GEMV_FULL, ctx);  // else recorded; nothing hangs
-      const uint8_t* stage = ring + st * S::STAGE;
-      if (ok && kb < p.kblocks) {
-        const uint8_t* x_at = stage + g * S::X_PITCH + wk * 256 + t * 16;
-        const uint8_t* blk[RT];
-        uint32_t w[RT][8];
+    for (int c = 0; c < chunks; c++) {
+      const int kb = c * S::WK + wk;
+      const bool ok = mbar_wait_soon(full + st, parity, SITE_GEMV_FULL, ctx);  // else recorded; nothing hangs
+      const uint8_t* stage = ring + st * p.stage_bytes;
+      auto block = [&](auto whole) {  // (behind K a stage holds whatever it held)
+        const uint8_t* x_at = stage + x_row + wk * 256 + t * 16;
+        const uint8_t* blk = stage + x_bytes + (wr * S::WK + wk) * S::BLOCK;  // of tile wr; the warp's next is WR further
+        constexpr int NEXT = WR * S::WK * S::BLOCK;
+        float acc[RT][4], one[4];
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-          blk[r] = stage + S::X_BYTES + ((wr * RT + r) * S::WK + wk) * p.block_bytes;
-          const uint4 lo = reinterpret_cast<const uint4*>(blk[r])[lane], hi = reinterpret_cast<const uint4*>(blk[r] + 512)[lane];
-          w[r][0] = lo.x; w[r][1] = lo.y; w[r][2] = lo.z; w[r][3] = lo.w;
-          w[r][4] = hi.x; w[r][5] = hi.y; w[r][6] = hi.z; w[r][7] = hi.w;
-        }
-        float acc[RT][NT][4], one[NT][4];
+        for (int half = 0; half < 2; half++) {
+          uint32_t w[RT][4];
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-          if ((2 * s) % steps_per_group == 0) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                one[n][i] = 0.0f;
-#pragma unroll
-                for (int r = 0; r < RT; r++) acc[r][n][i] = 0.0f;
-              }
+          for (int r = 0; r < RT; r++) {
+            const uint4 v = reinterpret_cast<const uint4*>(blk + r * NEXT + half * 512)[lane];
+            w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
           }
-          uint4 x[NT];
 #pragma unroll
-          for (int n = 0; n < NT; n++) x[n] = *reinterpret_cast<const uint4*>(x_at + n * 8 * S::X_PITCH + s * 64);
+          for (int s = 2 * half; s < 2 * half + 2; s++) {
+            const uint4 x = *reinterpret_cast<const uint4*>(x_at + s * 64);
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) mma_16816(one[n], ONES, ONES, ONES, ONES, e ? x[n].z : x[n].x, e ? x[n].w : x[n].y);
-#pragma unroll
-            for (int r = 0; r < RT; r++) {
-              const uint32_t a = w[r][2 * s + e], a2 = a >> 8;
-#pragma unroll
-              for (int n = 0; n < NT; n++)
-                mma_16816(acc[r][n], a & Q4_LO, a & Q4_HI, a2 & Q4_LO, a2 & Q4_HI, e ? x[n].z : x[n].x, e ? x[n].w : x[n].y);
-            }
-          }
-          if ((2 * s + 2) % steps_per_group == 0) {
-            const int in_block = (2 * s + 1) / steps_per_group;
-            if (kb * 128 + in_block * p.G < p.K) {  // (behind K a stage holds whatever it held)
+            for (int e = 0; e < 2; e++) {
+              const bool fresh = (2 * s + e) % GS == 0;
+              const uint32_t b0 = e ? x.z : x.x, b1 = e ? x.w : x.y;
+              if (fresh)
+                mma_16816_first(one, ONES, ONES, ONES, ONES, b0, b1);
+              else
+                mma_16816(one, ONES, ONES, ONES, ONES, b0, b1);
 #pragma unroll
               for (int r = 0; r < RT; r++) {
-                const __half2* par = reinterpret_cast<const __half2*>(blk[r] + 1024) + in_block * 16 + g;
-                const float2 lo = __half22float2(par[0]), hi = __half22float2(par[8]);
+                const uint32_t a = w[r][(2 * s + e) & 3], a2 = a >> 8;
+                if (fresh)
+                  mma_16816_first(acc[r], a & Q4_LO, a & Q4_HI, a2 & Q4_LO, a2 & Q4_HI, b0, b1);
+                else
+                  mma_16816(acc[r], a & Q4_LO, a & Q4_HI, a2 & Q4_LO, a2 & Q4_HI, b0, b1);
+              }
+            }
+            if ((2 * s + 2) % GS == 0) {
+              const int in_block = (2 * s + 1) / GS;
+              if (decltype(whole)::value || kb * 128 + in_block * (16 * GS) < p.K) {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int r = 0; r < RT; r++) {
+                  const __half2* par = reinterpret_cast<const __half2*>(blk + r * NEXT + 1024) + in_block * 16 + g;
+                  const float2 lo = __half22float2(par[0]), hi = __half22float2(par[8]);
 #pragma unroll
                   for (int i = 0; i < 2; i++) {
-                    y[r][n][i] = fmaf(lo.x, fmaf(-lo.y, one[n][i], acc[r][n][i] * Q4_LO_UNIT), y[r][n][i]);
-                    y[r][n][2 + i] = fmaf(hi.x, fmaf(-hi.y, one[n][i], acc[r][n][2 + i] * Q4_HI_UNIT), y[r][n][2 + i]);
+                    y[r][i] = fmaf(lo.x, fmaf(-lo.y, one[i], acc[r][i] * Q4_LO_UNIT), y[r][i]);
+                    y[r][2 + i] = fmaf(hi.x, fmaf(-hi.y, one[i], acc[r][2 + i] * Q4_HI_UNIT), y[r][2 + i]);
                   }
+                }
               }
             }
           }
         }
+      };
+      if (ok && kb < p.kblocks) {
+        if (kb * 128 + 128 <= p.K)
+          block(std::true_type{});
+        else
+          block(std::false_type{});
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + st);
+      if (++st == p.stages) {
+        st = 0;
+        parity ^= 1;
+      }
     }
     // ---- join the columns' warps, write ------------------------------------------------------------------------------------
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          out[(wk * S::COLS + n * 8 + 2 * t + (i & 1)) * S::OUT_PITCH + (wr * RT + r) * 16 + g + (i >> 1) * 8] = y[r][n][i];
+      for (int i = 0; i < 4; i++) out[(wk * 8 + 2 * t + (i & 1)) * S::OUT_PITCH + (r * WR + wr) * 16 + g + (i >> 1) * 8] = y[r][i];
     named_bar_sync(1, GV_WARPS * 32);
-    for (int i = threadIdx.x; i < S::COLS * S::ROWS; i += GV_WARPS * 32) {
-      const int row = i % S::ROWS, col = i / S::ROWS, m = m0 + col, n = tile0 * 16 + row;
-      if (m >= p.M) break;
-      if (n >= p.N) continue;
+    const int n_rows = min(min(S::TILES, last - tile0) * 16, p.N - tile0 * 16);
+    for (int i = threadIdx.x; i < n_m * S::ROWS; i += GV_WARPS * 32) {
+      const int row = i % S::ROWS, col = i / S::ROWS;
+      if (row >= n_rows) continue;
       float v = 0.0f;
 #pragma unroll
-      for (int k = 0; k < S::WK; k++) v += out[(k * S::COLS + col) * S::OUT_PITCH + row];
+      for (int k = 0; k < S::WK; k++) v += out[(k * 8 + col) * S::OUT_PITCH + row];
       v *= p.alpha;
-      const long long at = m * p.ldy + n;
+      const long long at = (m0 + col) * p.ldy + tile0 * 16 + row;
       if (p.out_f32) {
         float* o = static_cast<float*>(p.Y) + at;
         *o = p.beta == 0.0f ? v : fmaf(p.beta, *o, v);
@@ -280,67 +285,54 @@ int launch_q4_pack(const void* codes, long long ldc, const void* scales, long lo
 
 namespace {
 
-// CTAs of a kernel that share an SM, asked for once per device.
-template <int NT, int RT, int WR>
-cudaError_t per_sm_of(int* per_sm) {
-  using S = GemvShape<NT, RT, WR>;
-  auto kernel = gemv_q4_kernel<NT, RT, WR>;
-  static std::atomic<int> known[64];
+template <int RT, int WR, int GS>
+cudaError_t launch_shape(GemvParams& p, int sm_count, cudaStream_t stream) {
+  using S = GemvShape<RT, WR, GS>;
+  constexpr int MOST = 227 * 1024 / GV_PER_SM - 1024;  // bytes of a CTA
+  static std::atomic<bool> known[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  *per_sm = dev < 64 ? known[dev].load(std::memory_order_acquire) : 0;
-  if (*per_sm > 0) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kernel, GV_THREADS, S::SMEM);
-  if (e != cudaSuccess) return e;
-  *per_sm = *per_sm < 1 ? 1 : *per_sm;
-  if (dev < 64) known[dev].store(*per_sm, std::memory_order_release);
-  return cudaSuccess;
+  if (dev >= 64 || !known[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(gemv_q4_kernel<RT, WR, GS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) known[dev].store(true, std::memory_order_release);
+  }
+  const int room = MOST - S::HEAD - S::OUT;
+  static_assert((MOST - S::HEAD - S::OUT) / ((8 * S::X_PITCH + S::W_BYTES + 127) / 128 * 128) >= 2, "two stages at least");
+  p.stage_bytes = ((p.M < 8 ? p.M : 8) * S::X_PITCH + S::W_BYTES + 127) / 128 * 128;
+  p.stages = room / p.stage_bytes < S::MOST_STAGES ? room / p.stage_bytes : S::MOST_STAGES;
+  const int ctas = p.tiles < GV_PER_SM * sm_count ? p.tiles : GV_PER_SM * sm_count;
+  return launch_with_pdl(gemv_q4_kernel<RT, WR, GS>, dim3(ctas, (p.M + 7) / 8), dim3(GV_THREADS),
+                         S::HEAD + S::OUT + p.stages * p.stage_bytes, stream, p);
 }
 
-template <int NT, int RT, int WR>
-cudaError_t launch_shape(GemvParams& p, int sm_count, cudaStream_t stream) {
-  using S = GemvShape<NT, RT, WR>;
-  int per_sm = 0;
-  const cudaError_t e = per_sm_of<NT, RT, WR>(&per_sm);
-  if (e != cudaSuccess) return e;
-  p.row_groups = (p.tiles + S::TILES - 1) / S::TILES;
-  p.m_groups = (p.M + S::COLS - 1) / S::COLS;
-  const long long groups = static_cast<long long>(p.row_groups) * p.m_groups;
-  const long long room = static_cast<long long>(sm_count) * per_sm;
-  return launch_with_pdl(gemv_q4_kernel<NT, RT, WR>, dim3(static_cast<unsigned>(groups < room ? groups : room)), dim3(GV_THREADS),
-                         S::SMEM, stream, p);
-}
-
-// As many rows of W to a CTA as leave every SM one: fewer rows mean that more CTAs read X, more that some SMs have none.
-template <int NT>
-cudaError_t launch_rows_of(GemvParams& p, int sm_count, cudaStream_t stream) {
-  if constexpr (NT == 8) {
-    if (p.tiles >= 8 * sm_count) return launch_shape<NT, 1, 8>(p, sm_count, stream);
-    if (p.tiles >= 4 * sm_count) return launch_shape<NT, 1, 4>(p, sm_count, stream);
-  } else {
-    if (p.tiles >= 8 * sm_count) return launch_shape<NT, 2, 4>(p, sm_count, stream);
-    if (p.tiles >= 4 * sm_count) return launch_shape<NT, 2, 2>(p, sm_count, stream);
-  }
-  if constexpr (NT == 8) {  // (sixteen rows a CTA would leave no room for two stages)
-    return launch_shape<NT, 1, 2>(p, sm_count, stream);
-  } else {
-    if (p.tiles >= 2 * sm_count) return launch_shape<NT, 1, 2>(p, sm_count, stream);
-    return launch_shape<NT, 1, 1>(p, sm_count, stream);
-  }
+// The shape whose tiles are at least a CTA's share, so that its share is one pass over X.
+template <int GS>
+cudaError_t launch_group(GemvParams& p, int sm_count, cudaStream_t stream) {
+  const int share = (p.tiles + GV_PER_SM * sm_count - 1) / (GV_PER_SM * sm_count);
+  if (share <= 1) return launch_shape<1, 1, GS>(p, sm_count, stream);
+  if (share <= 2) return launch_shape<2, 1, GS>(p, sm_count, stream);
+  if (share <= 4) return launch_shape<2, 2, GS>(p, sm_count, stream);
+  if constexpr (GS == 2)
+    return launch_shape<2, 4, GS>(p, sm_count, stream);  // (four tiles a warp leave no room for two stages)
+  else
+    return launch_shape<4, 2, GS>(p, sm_count, stream);
 }
 
 }  // namespace
 
 int launch_gemv_q4(const void* X, long long ldx, const void* W, void* Y, long long ldy, int out_f32, int M, int N, int K,
                    int group, float alpha, float beta, int sm_count, uint32_t* status, cudaStream_t stream, const char** err) {
-  GemvParams p{static_cast<const __half*>(X), static_cast<const uint8_t*>(W), Y, ldx, ldy, M, N, K, group,
-               1024 + 64 * (128 / group), (K + 127) / 128, (N + 15) / 16, 0, 0, alpha, beta, out_f32, status};
-  cudaError_t e = M <= 8    ? launch_rows_of<1>(p, sm_count, stream)
-                  : M <= 16 ? launch_rows_of<2>(p, sm_count, stream)
-                  : M <= 32 ? launch_rows_of<4>(p, sm_count, stream)
-                            : launch_rows_of<8>(p, sm_count, stream);
+  if (M > 8 * 65535) {
+    *err = "gemv_q4: too many rows of X";
+    return -2;
+  }
+  GemvParams p{static_cast<const __half*>(X), static_cast<const uint8_t*>(W), Y, ldx, ldy, M, N, K, (K + 127) / 128,
+               (N + 15) / 16, 0, 0, alpha, beta, out_f32, status};
+  const cudaError_t e = group == 128  ? launch_group<8>(p, sm_count, stream)
+                        : group == 64 ? launch_group<4>(p, sm_count, stream)
+                                      : launch_group<2>(p, sm_count, stream);
   if (e == cudaSuccess) return 0;
   *err = cudaGetErrorString(e);
   return -3;

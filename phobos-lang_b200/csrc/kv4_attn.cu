@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : 1) kv4_attn_kerne
 #pragma unroll 1
       for (int i = 0; i < n_tiles; i++) {
         const uint32_t n = phase + i, st = n % STAGES, here = (present >> (st * UN)) & ((1u << UN) - 1);
-        if (!mbar_wait_warp(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx)) continue;  // recorded; nothing hangs
+        if (!mbar_wait_soon(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx)) continue;  // recorded; nothing hangs
         const int tok0 = (w0 + i * UN) * KV4_UNIT;
         const uint8_t* stage = ring + st * S::STAGE;
         if (tok0 >= all_lo && tok0 + UN * KV4_UNIT <= all_hi && here == (1u << UN) - 1)
