@@ -16,7 +16,7 @@ CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 LIB = HERE / "libphobos_leaf.so"
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_f32.cu", "flash.cu", "elementwise.cu", "kda.cu", "tmap.cu", "noalloc.cu", "selftest.cu",
-           "gemv_q4.cu", "kv4_cache.cu", "kv4_attn.cu", "kv4_pages.cu", "serve_api.cu",
+           "gemv_q4.cu", "gemv_q4_tc.cu", "kv4_cache.cu", "kv4_attn.cu", "kv4_pages.cu", "serve_api.cu",
            "host.cpp", "executor.cpp", "source.cpp", "planner.cpp", "plan_api.cpp", "wire.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-Xptxas", "-v"]

@@ -324,6 +324,8 @@ cudaError_t launch_group(GemvParams& p, int sm_count, cudaStream_t stream) {
 
 int launch_gemv_q4(const void* X, long long ldx, const void* W, void* Y, long long ldy, int out_f32, int M, int N, int K,
                    int group, float alpha, float beta, int sm_count, uint32_t* status, cudaStream_t stream, const char** err) {
+  if (M > 8 && gemv_q4_tc_is_faster(M, N, K, group, sm_count))
+    return launch_gemv_q4_tc(X, ldx, W, Y, ldy, out_f32, M, N, K, group, alpha, beta, sm_count, status, stream, err);
   if (M > 8 * 65535) {
     *err = "gemv_q4: too many rows of X";
     return -2;

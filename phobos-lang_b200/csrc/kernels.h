@@ -95,6 +95,12 @@ int launch_q4_pack(const void* codes, long long ldc, const void* scales, long lo
 int launch_gemv_q4(const void* X, long long ldx, const void* W, void* Y, long long ldy, int out_f32, int M, int N, int K,
                    int group, float alpha, float beta, int sm_count, uint32_t* status, cudaStream_t stream, const char** err);
 
+// gemv_q4_tc.cu — the same for more than eight rows of X, on tcgen05, and whether its times are expected below those of
+// gemv_q4.cu's kernel run for eight rows at a time.
+bool gemv_q4_tc_is_faster(int M, int N, int K, int group, int sm_count);
+int launch_gemv_q4_tc(const void* X, long long ldx, const void* W, void* Y, long long ldy, int out_f32, int M, int N, int K,
+                      int group, float alpha, float beta, int sm_count, uint32_t* status, cudaStream_t stream, const char** err);
+
 // The 4-bit key/value cache (layout in kv4.cuh): one layer of it for the kernels that read or write tokens.
 struct Kv4View {
   uint8_t* pages;       // this layer's pages

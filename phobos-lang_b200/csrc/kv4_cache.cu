@@ -1,8 +1,10 @@
 // Rows of keys and values into the 4-bit cache, and back.
 //
 //   scale = f16((max - min) / 15), zero = min, code = rint((x - min) / scale) in 0..15     per group of G dims
-// Differences and quotients are f32 with IEEE rounding, so the codes do not depend on how the work is split.  A group
-// whose range rounds to a scale of zero holds `zero` alone; a group with a value that is not finite reads back as NaN.
+// The codes are found without a division: k = rint((x - min) * (1 / scale)) is right unless the product lies close to the
+// middle between two codes; then e = (x - min) - k scale, which f32 holds exactly, says whether it is, and at e = scale / 2
+// which neighbour is even.  (With a division for each value 24000 rows of 8 x 128 took 186 us, bound by instructions.)  A
+// group whose range rounds to a scale of zero holds `zero` alone; a group with a value that is not finite reads back as NaN.
 #include "kv4.cuh"
 
 namespace ph {
@@ -21,122 +23,223 @@ struct RowParams {
   uint32_t* status;
 };
 
-constexpr int ROW_THREADS = 128;
+constexpr int ROW_WARPS = 8;
 
-// One warp: a row and one head of it (D = 128), or a row and two heads (D = 64).
+constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: a sum's low bits are the other number, rounded
+
+// rint(a / s) for a >= 0, s > 0 and quotients below 2^21, at most 15.
+__device__ __forceinline__ uint32_t code_of(float a, float s, float per_s) {
+  const float m = fmaf(a, per_s, MAGIC);
+  int k = static_cast<int>(__float_as_uint(m) & 0x3fffffu);
+  const float e = fmaf(-(m - MAGIC), s, a), off = fabsf(e), half = 0.5f * s;
+  if (off > half || (off == half && (k & 1))) k += e > 0.0f ? 1 : -1;
+  return static_cast<uint32_t>(min(k, 15));
+}
+
+// Which unit of which sequence a CTA works on.
+struct Job {
+  Kv4Rows rows;
+  int unit;  // of the sequence; below 0 for rows whose token is not in the cache
+};
+
+// A sequence's new tokens stand in units (length - rows) / 16 .. (length - 1) / 16, rounded down.
+__device__ __forceinline__ int units_of(const Kv4Rows& r, int* first) {
+  const int n = r.end - r.begin;
+  *first = (r.length - n) >> 4;
+  return n > 0 ? ((r.length - 1) >> 4) - *first + 1 : 0;
+}
+
+// The job of CTA `at`: the sequences are walked a CTA's width at a time.  False behind the last.
+__device__ bool find_job(const RowParams& p, int at, Job* job) {
+  __shared__ int warp_sum[ROW_WARPS];
+  __shared__ Job found;
+  int first;
+  if (!p.ind) {  // one row, so one unit each
+    if (at >= p.n) return false;
+    job->rows = kv4_rows(p.c, p.slots, p.ind, at, p.T, p.status);
+    units_of(job->rows, &first);
+    job->unit = first;
+    return true;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int done = 0;
+  for (int i0 = 0; i0 < p.n; i0 += ROW_WARPS * 32) {
+    const int b = i0 + threadIdx.x;
+    int count = 0;
+    Kv4Rows rows{};
+    if (b < p.n) {
+      rows = kv4_rows(p.c, p.slots, p.ind, b, p.T, p.status);
+      count = units_of(rows, &first);
+    }
+    int sum = count;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    int before = done, total = 0;
+    for (int w = 0; w < ROW_WARPS; w++) {
+      if (w < warp) before += warp_sum[w];
+      total += warp_sum[w];
+    }
+    before += sum - count;
+    if (at >= before && at < before + count) {
+      found.rows = rows;
+      found.unit = first + at - before;
+    }
+    done += total;
+    __syncthreads();
+    if (at < done) break;
+  }
+  if (at >= done) return false;
+  *job = found;
+  return true;
+}
+
+// One CTA: a unit of one sequence; each warp takes heads in turn.  D / 8 lanes work on a row's key and D / 8 on its value,
+// eight dims each, in as many rows at once as a warp holds.  A unit whose sixteen tokens are all there goes through shared
+// memory and is read or written in one piece of 16-byte words; of any other one only the rows' own bytes are touched.
 template <int D, bool READ>
-__global__ void __launch_bounds__(ROW_THREADS) kv4_rows_kernel(RowParams p) {
-  constexpr int W = D / 8, PER = 32 / (2 * W);  // lanes of a key or value; heads of a warp
-  const int lane = threadIdx.x & 31;
-  const int head_groups = (p.c.heads + PER - 1) / PER;
-  const long long job = static_cast<long long>(blockIdx.x) * (ROW_THREADS / 32) + (threadIdx.x >> 5);
-  if (job >= static_cast<long long>(p.T) * head_groups) return;
-  const int row = static_cast<int>(job / head_groups), hg = static_cast<int>(job % head_groups);
-  const int b = kv4_find(p.ind, p.n, row);
-  const Kv4Rows rows = kv4_rows(p.c, p.slots, p.ind, b, p.T, p.status);
-  const int pos = rows.length - (rows.end - rows.begin) + (row - rows.begin);
-  if (row < rows.begin || row >= rows.end) return;  // rows behind the last sequence stay as they are
-  const int head = hg * PER + lane / (2 * W);
+__global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p) {
+  constexpr int W = D / 8, AT_ONCE = 32 / (2 * W), PASSES = KV4_UNIT / AT_ONCE, AHEAD = 4;
+  __shared__ __align__(16) uint8_t image[ROW_WARPS][16 * D + 128 * (D / 32)];
+  Job job;
+  if (!find_job(p, blockIdx.x, &job)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = job.rows.end - job.rows.begin, first = job.rows.length - n;
+  const int r0 = max(first - job.unit * 16, 0), r1 = min(job.rows.length - job.unit * 16, 16);  // its tokens r0 .. r1 - 1 are rows
+  const bool whole = r0 == 0 && r1 == 16;
+  const int page = job.unit >= 0 ? kv4_page(p.c, job.rows.slot, job.unit * 16, p.status) : -1;
+  const int groups = D / p.c.G, unit_bytes = kv4_unit_bytes(D, p.c.G), page_units = 1 << (p.c.page_shift - 4);
   const bool value = (lane % (2 * W)) >= W;
-  const int word = lane % W;
-  const bool live = head < p.c.heads;
-  int page = -1;
-  if (pos >= 0) page = kv4_page(p.c, rows.slot, pos, p.status);
-  const int groups = D / p.c.G, grp = word * 8 / p.c.G;
-  const int r = pos & 15, unit_bytes = kv4_unit_bytes(D, p.c.G), page_units = 1 << (p.c.page_shift - 4);
-  uint8_t* unit = p.c.pages + page * p.c.page_bytes +
-                  (static_cast<long long>(head) * page_units + ((pos & ((1 << p.c.page_shift) - 1)) >> 4)) * unit_bytes;
-  // where this lane's eight codes and its group's pair stand in the unit
-  const int k_at = (r >> 3) * 4 * D + ((r & 7) * 4 + (word & 3)) * W + (word >> 2) * 4;
-  const int v_at = 8 * D + (r >> 3) * 4 * D + (2 * (word & 3) * 4 + ((r & 7) >> 1)) * W + (word >> 2) * 4 + (r & 1) * 2;
-  const int par_at = 16 * D + (value ? 64 * groups : 0) + (r * groups + grp) * 4;
-  const long long at = row * (value ? p.ldv : p.ldk) + head * D + word * 8;
-  if constexpr (READ) {
-    if (!live) return;
-    uint4 out = make_uint4(0, 0, 0, 0);  // a row whose token is not in the cache reads as zero
-    if (page >= 0) {
-      uint32_t codes;
-      if (value)
-        codes = *reinterpret_cast<const uint16_t*>(unit + v_at) |
-                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit + v_at + 4 * W)) << 16;
-      else
-        codes = *reinterpret_cast<const uint32_t*>(unit + k_at);
-      const float2 sz = __half22float2(*reinterpret_cast<const __half2*>(unit + par_at));
-      float x[8];
+  const int word = lane % W, grp = word * 8 / p.c.G;
+  for (int head = warp; head < p.c.heads; head += ROW_WARPS) {
+    uint8_t* unit = p.c.pages + page * p.c.page_bytes +
+                    (static_cast<long long>(head) * page_units + (job.unit & (page_units - 1))) * unit_bytes;
+    uint8_t* to = whole ? image[warp] : unit;
+    if (READ && whole && page >= 0) {
+      __syncwarp();
+      for (int i = lane; i < unit_bytes / 16; i += 32)
+        reinterpret_cast<uint4*>(image[warp])[i] = reinterpret_cast<const uint4*>(unit)[i];
+      __syncwarp();
+    }
+    uint4 rows[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[i] = fmaf(sz.x, static_cast<float>((codes >> (4 * i)) & 15u), sz.y);
-        // zero + 15 scale can pass the group's maximum by half a step of the f16 scale: not into infinity (NaN stays)
-        if (x[i] > 65504.0f) x[i] = 65504.0f;
-        if (x[i] < -65504.0f) x[i] = -65504.0f;
+    for (int k = 0; k < PASSES; k++) {
+      const int r = k * AT_ONCE + lane / (2 * W);
+      const bool live = r >= r0 && r < r1;
+      if constexpr (!READ) {
+        if (k % AHEAD == 0) {
+#pragma unroll
+          for (int i = 0; i < AHEAD; i++) {
+            const int ri = r + i * AT_ONCE;
+            rows[i] = make_uint4(0, 0, 0, 0);
+            if (ri >= r0 && ri < r1)
+              rows[i] = *reinterpret_cast<const uint4*>((value ? p.V : p.K) + (job.rows.begin + job.unit * 16 + ri - first) * (value ? p.ldv : p.ldk) +
+                                                        head * D + word * 8);
+          }
+        }
       }
-      __half2* o = reinterpret_cast<__half2*>(&out);
+      if (!whole && !__any_sync(0xffffffffu, live)) continue;
+      // where this lane's eight codes and its group's pair stand in the unit
+      const int k_at = (r >> 3) * 4 * D + ((r & 7) * 4 + (word & 3)) * W + (word >> 2) * 4;
+      const int v_at = 8 * D + (r >> 3) * 4 * D + (2 * (word & 3) * 4 + ((r & 7) >> 1)) * W + (word >> 2) * 4 + (r & 1) * 2;
+      const int par_at = 16 * D + (value ? 64 * groups : 0) + (r * groups + grp) * 4;
+      if constexpr (READ) {
+        if (!live) continue;
+        uint4 out = make_uint4(0, 0, 0, 0);  // a row whose token is not in the cache reads as zero
+        if (page >= 0) {
+          uint32_t codes;
+          if (value)
+            codes = *reinterpret_cast<const uint16_t*>(to + v_at) |
+                    static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(to + v_at + 4 * W)) << 16;
+          else
+            codes = *reinterpret_cast<const uint32_t*>(to + k_at);
+          const float2 sz = __half22float2(*reinterpret_cast<const __half2*>(to + par_at));
+          float x[8];
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    }
-    *reinterpret_cast<uint4*>((value ? p.Vout : p.Kout) + at) = out;
-  } else {
-    uint4 in = make_uint4(0, 0, 0, 0);
-    if (live) in = *reinterpret_cast<const uint4*>((value ? p.V : p.K) + at);
-    const __half2* h = reinterpret_cast<const __half2*>(&in);
-    float x[8];
+          for (int i = 0; i < 8; i++) {
+            x[i] = fmaf(sz.x, static_cast<float>((codes >> (4 * i)) & 15u), sz.y);
+            // zero + 15 scale can pass the group's maximum by half a step of the f16 scale: not into infinity (NaN stays)
+            if (x[i] > 65504.0f) x[i] = 65504.0f;
+            if (x[i] < -65504.0f) x[i] = -65504.0f;
+          }
+          __half2* o = reinterpret_cast<__half2*>(&out);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 f = __half22float2(h[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-    float lo = x[0], hi = x[0];
-    bool finite = true;
+          for (int i = 0; i < 4; i++) o[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        }
+        *reinterpret_cast<uint4*>((value ? p.Vout : p.Kout) + (job.rows.begin + job.unit * 16 + r - first) * (value ? p.ldv : p.ldk) + head * D +
+                                  word * 8) = out;
+      } else {
+        // the group's minimum and, negated, its maximum in one pair; NaN wins
+        const __half2* h = reinterpret_cast<const __half2*>(&rows[k % AHEAD]);
+        const __half2 even_odd = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
+        const __half2 neg = __hmin2_nan(__hmin2_nan(__hneg2(h[0]), __hneg2(h[1])), __hmin2_nan(__hneg2(h[2]), __hneg2(h[3])));
+        __half2 ends = __hmin2_nan(__lows2half2(even_odd, neg), __highs2half2(even_odd, neg));
+        for (int d = 1; d < p.c.G / 8; d *= 2) ends = __hmin2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, d));  // its lanes are neighbours
+        if (!live || page < 0) continue;
+        const float lo = __low2float(ends), range = __fsub_rn(-__high2float(ends), lo);
+        const bool bad = !(range <= 2.0f * 65504.0f);
+        const __half scale = __float2half_rn(__fdiv_rn(range, 15.0f));
+        const float s = __half2float(scale);
+        uint32_t codes = 0;
+        if (s > 0.0f && !bad) {
+          float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      finite = finite && fabsf(x[i]) <= 65504.0f;
-    }
-    int bad = finite ? 0 : 1;
-    for (int d = 1; d < p.c.G / 8; d *= 2) {  // the group's lanes are neighbours
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-      bad |= __shfl_xor_sync(0xffffffffu, bad, d);
-    }
-    if (!live || page < 0) return;
-    const __half scale = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
-    const float s = __half2float(scale);
-    uint32_t codes = 0;
-    if (s > 0.0f && !bad) {
+          for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(h[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+          }
+          const float per_s = 1.0f / s;
+          float off = range * per_s > 15.4f ? 1.0f : 0.0f;  // (a subnormal scale's error can lead past 15)
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], lo), s)), 0.0f), 15.0f);
-        codes |= static_cast<uint32_t>(c) << (4 * i);
+          for (int i = 7; i >= 0; i--) {
+            const float a = __fsub_rn(x[i], lo), m = fmaf(a, per_s, MAGIC);
+            off = fmaxf(off, fabsf(fmaf(a, per_s, MAGIC - m)));
+            codes = codes << 4 | (__float_as_uint(m) & 15u);
+          }
+          if (off > 0.499f) {
+            codes = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) codes |= code_of(__fsub_rn(x[i], lo), s, per_s) << (4 * i);
+          }
+        }
+        if (value) {
+          *reinterpret_cast<uint16_t*>(to + v_at) = static_cast<uint16_t>(codes);
+          *reinterpret_cast<uint16_t*>(to + v_at + 4 * W) = static_cast<uint16_t>(codes >> 16);
+        } else {
+          *reinterpret_cast<uint32_t*>(to + k_at) = codes;
+        }
+        if (word * 8 % p.c.G == 0) {
+          const __half nan = __ushort_as_half(0x7e00);
+          *reinterpret_cast<__half2*>(to + par_at) = bad ? __halves2half2(nan, nan) : __halves2half2(scale, __float2half_rn(lo));
+        }
       }
     }
-    if (value) {
-      *reinterpret_cast<uint16_t*>(unit + v_at) = static_cast<uint16_t>(codes);
-      *reinterpret_cast<uint16_t*>(unit + v_at + 4 * W) = static_cast<uint16_t>(codes >> 16);
-    } else {
-      *reinterpret_cast<uint32_t*>(unit + k_at) = codes;
-    }
-    if (word * 8 % p.c.G == 0) {
-      const __half nan = __ushort_as_half(0x7e00);
-      *reinterpret_cast<__half2*>(unit + par_at) = bad ? __halves2half2(nan, nan) : __halves2half2(scale, __float2half_rn(lo));
+    if (!READ && whole && page >= 0) {
+      __syncwarp();
+      for (int i = lane; i < unit_bytes / 16; i += 32)
+        reinterpret_cast<uint4*>(unit)[i] = reinterpret_cast<const uint4*>(image[warp])[i];
+      __syncwarp();
     }
   }
 }
 
 template <bool READ>
 int launch_rows(const RowParams& p, cudaStream_t stream, const char** err) {
-  const int per = p.c.D == 128 ? 1 : 2;
-  const long long jobs = static_cast<long long>(p.T) * ((p.c.heads + per - 1) / per);
-  const long long blocks = (jobs + ROW_THREADS / 32 - 1) / (ROW_THREADS / 32);
-  if (blocks > 0x7fffffffLL) {
+  // an upper bound on the units that the rows stand in: a sequence's first and last may be partly theirs
+  const long long jobs = p.ind ? static_cast<long long>(p.T) / KV4_UNIT + 2LL * p.n : p.n;
+  if (jobs > 0x7fffffffLL) {
     *err = "kv4: too many rows";
     return -2;
   }
   if (p.c.D == 128)
-    kv4_rows_kernel<128, READ><<<static_cast<unsigned>(blocks), ROW_THREADS, 0, stream>>>(p);
+    kv4_rows_kernel<128, READ><<<static_cast<unsigned>(jobs), ROW_WARPS * 32, 0, stream>>>(p);
   else
-    kv4_rows_kernel<64, READ><<<static_cast<unsigned>(blocks), ROW_THREADS, 0, stream>>>(p);
+    kv4_rows_kernel<64, READ><<<static_cast<unsigned>(jobs), ROW_WARPS * 32, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return 0;
   *err = cudaGetErrorString(e);

@@ -34,7 +34,9 @@ def _tol(S, y, K, G, half):
 
 CASES = [(1, 16, 128, 128), (1, 1, 32, 32), (2, 17, 96, 32), (3, 130, 64, 64), (5, 33, 320, 64), (7, 8, 1152, 128), (8, 257, 2048, 128),
          (9, 100, 416, 32), (16, 64, 4096, 64), (17, 200, 640, 128), (33, 48, 1024, 32), (64, 96, 512, 128), (65, 31, 256, 64), (200, 40, 128, 128),
-         (1, 4100, 1024, 128), (4, 2500, 8192, 64), (1, 24, 16384, 32)]
+         (1, 4100, 1024, 128), (4, 2500, 8192, 64), (1, 24, 16384, 32),
+         # sizes at which the tensor-core form is taken: each width of it, rows shared out along K, several groups of rows, a ragged K
+         (11, 16387, 8192, 128), (30, 16011, 4096, 64), (64, 4100, 4096, 128), (200, 3001, 2048, 128), (61, 16500, 1056, 32)]
 
 
 @pytest.mark.parametrize("M,N,K,G", CASES)
