@@ -335,7 +335,7 @@ struct AttnShape {
 };
 
 template <int D, int NG, int NT, int UN, int STAGES>
-__global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : 1) kv4_attn_kernel(AttnParams p) {
+__global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) kv4_attn_kernel(AttnParams p) {
   using S = AttnShape<D, NG, NT, UN, STAGES>;
   constexpr int J = D / 32, ROWS = S::ROWS;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -396,31 +396,32 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : 1) kv4_attn_kerne
       // ---- its units in this piece, their pages, and the first tiles under way ----------------------------------------------
       const int last_row = min(row0 + ROWS, n_rows) - 1;
       const int visible = (max(first + last_row / p.rep + 1, 0) + KV4_UNIT - 1) / KV4_UNIT;  // units that hold a seen token
-      const int w0 = u_begin + from, w1 = min(u_begin + upto, visible);
-      int page_base = w0, page_id = -1;  // lane i knows the page of unit page_base + i
-      auto look_up = [&](int base) {
-        page_base = base;
-        page_id = base + lane < w1 ? kv4_page(p.c, rows.slot, (base + lane) * KV4_UNIT, p.status) : -1;
+      // (units before the window of the tile's first row, whose sequence's earliest row may reach further back, are left out)
+      const int window_begin = p.a.window > 0 ? max(first + row0 / p.rep + 1 - p.a.window, 0) / KV4_UNIT : 0;
+      const int w0 = max(u_begin + from, window_begin), w1 = min(u_begin + upto, visible);
+      int base = w0;                     // lane i knows where unit base + i is, and copies it
+      const uint8_t* source = nullptr;   // (null: not there)
+      auto look_up = [&](int from_unit) {
+        base = from_unit;
+        const int u = base + lane, page = u < w1 ? kv4_page(p.c, rows.slot, u * KV4_UNIT, p.status) : -1;
+        source = page < 0 ? nullptr
+                          : p.c.pages + page * p.c.page_bytes +
+                                (static_cast<long long>(head) * page_units + (u & (page_units - 1))) * S::UNIT;
       };
-      auto issue = [&](int u, uint32_t at_tile) {  // units [u, u + UN) into the tile's stage; returns which are there
-        if (u + UN > page_base + 32) look_up(u);
-        const int page = __shfl_sync(0xffffffffu, page_id, (u - page_base + lane) & 31);
-        const bool is = lane < UN && u + lane < w1 && page >= 0;
-        const uint32_t present = __ballot_sync(0xffffffffu, is);
-        const int st = at_tile % STAGES;
+      auto issue = [&](int u, uint32_t st) {  // units [u, u + UN) into a stage; returns which are there
+        if (u + UN > base + 32) look_up(u);
+        const int of = u - base, k = lane - of;
+        const bool is = k >= 0 && k < UN && source != nullptr;
+        const uint32_t present = __ballot_sync(0xffffffffu, is) >> of;
         if (lane == 0) mbar_arrive_expect_tx(bar + st, __popc(present) * S::UNIT);
         __syncwarp();
-        if (is)
-          bulk_load(ring + st * S::STAGE + lane * S::UNIT,
-                    p.c.pages + page * p.c.page_bytes +
-                        (static_cast<long long>(head) * page_units + ((u + lane) & (page_units - 1))) * S::UNIT,
-                    S::UNIT, bar + st);
+        if (is) bulk_load(ring + st * S::STAGE + k * S::UNIT, source, S::UNIT, bar + st);
         return present;
       };
       const int n_tiles = w0 < w1 ? (w1 - w0 + UN - 1) / UN : 0;
       if (n_tiles > 0) look_up(w0);
       uint32_t present = 0;  // UN bits a stage
-      for (int k = 0; k < STAGES && k < n_tiles; k++) present |= issue(w0 + k * UN, phase + k) << ((phase + k) % STAGES * UN);
+      for (int k = 0; k < STAGES && k < n_tiles; k++) present |= issue(w0 + k * UN, (phase + k) % STAGES) << ((phase + k) % STAGES * UN);
       // ---- queries -------------------------------------------------------------------------------------------------------
       Queries<D, NG, NT> q;
 #pragma unroll
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : 1) kv4_attn_kerne
         __syncwarp();
         if (i + STAGES < n_tiles) {
           present &= ~(((1u << UN) - 1) << (st * UN));
-          present |= issue(w0 + (i + STAGES) * UN, n + STAGES) << (st * UN);
+          present |= issue(w0 + (i + STAGES) * UN, st) << (st * UN);
         }
       }
       phase += n_tiles;
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : 1) kv4_attn_kerne
   }
 }
 
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 512;
 
 // Joins the parts of problems that were cut.  An item is every `split`-th row of one problem; CTA b looks at items b,
 // b + gridDim.x, ... all at once, for most pieces end without a cut, and joins those that there are.
@@ -688,7 +689,7 @@ cudaError_t launch_attn(AttnParams& p, int most_rows, int sm_count, cudaStream_t
 
 template <int D, int NG>
 cudaError_t launch_rows_of(AttnParams& p, int nt, int most_rows, int sm_count, cudaStream_t stream) {
-  return nt == 1 ? launch_attn<D, NG, 1, 4, 2>(p, most_rows, sm_count, stream) : launch_attn<D, NG, 2, 2, 3>(p, most_rows, sm_count, stream);
+  return nt == 1 ? launch_attn<D, NG, 1, 4, 2>(p, most_rows, sm_count, stream) : launch_attn<D, NG, 2, 2, 2>(p, most_rows, sm_count, stream);
 }
 
 // Rows of a problem: eight where every sequence brings at most eight rows a key/value head, sixteen otherwise.

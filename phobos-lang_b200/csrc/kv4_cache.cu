@@ -105,6 +105,7 @@ template <int D, bool READ>
 __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p) {
   constexpr int W = D / 8, AT_ONCE = 32 / (2 * W), PASSES = KV4_UNIT / AT_ONCE, AHEAD = 4;
   __shared__ __align__(16) uint8_t image[ROW_WARPS][16 * D + 128 * (D / 32)];
+  pdl_wait();
   Job job;
   if (!find_job(p, blockIdx.x, &job)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -236,11 +237,8 @@ int launch_rows(const RowParams& p, cudaStream_t stream, const char** err) {
     *err = "kv4: too many rows";
     return -2;
   }
-  if (p.c.D == 128)
-    kv4_rows_kernel<128, READ><<<static_cast<unsigned>(jobs), ROW_WARPS * 32, 0, stream>>>(p);
-  else
-    kv4_rows_kernel<64, READ><<<static_cast<unsigned>(jobs), ROW_WARPS * 32, 0, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_with_pdl(p.c.D == 128 ? kv4_rows_kernel<128, READ> : kv4_rows_kernel<64, READ>, dim3(static_cast<unsigned>(jobs)),
+                                        dim3(ROW_WARPS * 32), 0, stream, p);
   if (e == cudaSuccess) return 0;
   *err = cudaGetErrorString(e);
   return -3;

@@ -127,6 +127,8 @@ __device__ long long scan_fresh(const Plan& p, int n) {
 
 __global__ void __launch_bounds__(PLAN_THREADS) extend_plan_kernel(Kv4View c, Plan p, const int* slots, const int* counts, int n,
                                                                    int* shortfall) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ int wrong, moves;
   if (threadIdx.x == 0) {
     wrong = 0;
@@ -210,6 +212,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_plan_kernel(Kv4View c, Pl
 
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Kv4View c, Plan p, const int* src, const int* dst, int n,
                                                                  int deep, int* shortfall) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ int wrong;
   if (threadIdx.x == 0) {
     wrong = 0;
@@ -276,6 +280,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Kv4View c, Plan
 
 // One CTA per row: gives back the pages behind the first `keep` tokens.
 __global__ void __launch_bounds__(MOVE_THREADS) free_kernel(Kv4View c, const int* slots, const int* keep, int n) {
+  pdl_wait();
+  pdl_launch_dependents();
   const int i = blockIdx.x, slot = slots[i];
   if (slot < 0 || slot >= c.max_seqs) return;
   int earlier = 0;  // a sequence that is named twice goes by its first row
@@ -296,6 +302,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) free_kernel(Kv4View c, const int
 
 // With L live pages: the live pages at L and above, in order, go to the free places below L, in order.
 __global__ void __launch_bounds__(PLAN_THREADS) compact_plan_kernel(Kv4View c, Plan p, int* live_out) {
+  pdl_wait();
+  pdl_launch_dependents();
   int live = 0;
   for (int i0 = 0; i0 < c.n_pages; i0 += PLAN_THREADS) {
     const int i = i0 + threadIdx.x;
@@ -329,6 +337,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_plan_kernel(Kv4View c, P
 
 // Tables after a compaction: pages at L (= *live) and above have moved.
 __global__ void __launch_bounds__(MOVE_THREADS) remap_kernel(Kv4View c, Plan p, const int* live) {
+  pdl_wait();
+  pdl_launch_dependents();
   const int l = *live;
   for (int slot = blockIdx.x; slot < c.max_seqs; slot += gridDim.x) {
     const int used = min(pages_for(c, max(c.lens[slot], 0)), c.table_width);
@@ -342,6 +352,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) remap_kernel(Kv4View c, Plan p, 
 
 // Moves pages of every layer; the list and its length come from the plan.  An item is 16 KB of one page.
 __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(Kv4View c, const int* n_moves, const int2* moves) {
+  pdl_wait();
+  pdl_launch_dependents();
   constexpr int ITEM = 16384;
   const int chunks = static_cast<int>((c.page_bytes + ITEM - 1) / ITEM);
   const long long items = static_cast<long long>(*n_moves) * c.layers * chunks;
@@ -364,16 +376,21 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(Kv4View c, const int
   }
 }
 
-int launched(const char** err) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return 0;
-  *err = cudaGetErrorString(e);
-  return -3;
-}
-
-void move(const Kv4View& c, const Plan& p, int sm_count, cudaStream_t stream) {
-  move_kernel<<<sm_count * 8, MOVE_THREADS, 0, stream>>>(c, p.n_moves, p.moves);
-}
+// Launches one after another; nothing more once one has failed.
+struct Launches {
+  cudaStream_t stream;
+  cudaError_t error = cudaSuccess;
+  template <typename... KArgs, typename... Args>
+  void add(void (*kernel)(KArgs...), int blocks, int threads, Args... args) {
+    if (error == cudaSuccess) error = launch_with_pdl(kernel, dim3(blocks), dim3(threads), 0, stream, args...);
+  }
+  void move(const Kv4View& c, const Plan& p, int sm_count) { add(move_kernel, sm_count * 8, MOVE_THREADS, c, p.n_moves, p.moves); }
+  int done(const char** err) const {
+    if (error == cudaSuccess) return 0;
+    *err = cudaGetErrorString(error);
+    return -3;
+  }
+};
 
 }  // namespace
 
@@ -385,30 +402,34 @@ size_t kv4_pages_workspace(const Kv4View& c) {
 int launch_kv4_extend(const Kv4View& c, const int* slots, const int* counts, int n, int* shortfall, void* workspace,
                       int sm_count, cudaStream_t stream, const char** err) {
   const Plan p = plan_of(c, workspace);
-  extend_plan_kernel<<<1, PLAN_THREADS, 0, stream>>>(c, p, slots, counts, n, shortfall);
-  move(c, p, sm_count, stream);
-  return launched(err);
+  Launches l{stream};
+  l.add(extend_plan_kernel, 1, PLAN_THREADS, c, p, slots, counts, n, shortfall);
+  l.move(c, p, sm_count);
+  return l.done(err);
 }
 
 int launch_kv4_fork(const Kv4View& c, const int* src, const int* dst, int n, int deep, int* shortfall, void* workspace,
                     int sm_count, cudaStream_t stream, const char** err) {
   const Plan p = plan_of(c, workspace);
-  fork_plan_kernel<<<1, PLAN_THREADS, 0, stream>>>(c, p, src, dst, n, deep, shortfall);
-  if (deep) move(c, p, sm_count, stream);
-  return launched(err);
+  Launches l{stream};
+  l.add(fork_plan_kernel, 1, PLAN_THREADS, c, p, src, dst, n, deep, shortfall);
+  if (deep) l.move(c, p, sm_count);
+  return l.done(err);
 }
 
 int launch_kv4_free(const Kv4View& c, const int* slots, const int* keep, int n, cudaStream_t stream, const char** err) {
-  free_kernel<<<n, MOVE_THREADS, 0, stream>>>(c, slots, keep, n);
-  return launched(err);
+  Launches l{stream};
+  l.add(free_kernel, n, MOVE_THREADS, c, slots, keep, n);
+  return l.done(err);
 }
 
 int launch_kv4_compact(const Kv4View& c, int* live, void* workspace, int sm_count, cudaStream_t stream, const char** err) {
   const Plan p = plan_of(c, workspace);
-  compact_plan_kernel<<<1, PLAN_THREADS, 0, stream>>>(c, p, live);
-  move(c, p, sm_count, stream);
-  remap_kernel<<<c.max_seqs < 4 * sm_count ? c.max_seqs : 4 * sm_count, MOVE_THREADS, 0, stream>>>(c, p, live);
-  return launched(err);
+  Launches l{stream};
+  l.add(compact_plan_kernel, 1, PLAN_THREADS, c, p, live);
+  l.move(c, p, sm_count);
+  l.add(remap_kernel, c.max_seqs < 4 * sm_count ? c.max_seqs : 4 * sm_count, MOVE_THREADS, c, p, live);
+  return l.done(err);
 }
 
 }  // namespace ph

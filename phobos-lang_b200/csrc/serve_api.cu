@@ -230,11 +230,11 @@ int phobos_kv4_attention(const PhKv4Cache* cache, int32_t layer, const PhTensor*
   if (window < 0) return fail(PH_ERR_INVALID, "kv4_attention: window %d", window);
   if ((rc = batch_of("kv4_attention", slots, indptr, n, q.rows))) return rc;
   const long long T = indptr ? q.rows : n;
+  const size_t need = kv4_attention_workspace(c, static_cast<int>(T), n, static_cast<int>(q_heads), sm_count_or_default());
+  if ((rc = workspace_of("kv4_attention", workspace, workspace_bytes, need))) return rc;
   int sms;
   uint32_t* status;
   if ((rc = device_props(&sms, &status))) return rc;
-  const size_t need = kv4_attention_workspace(c, static_cast<int>(T), n, static_cast<int>(q_heads), sms);
-  if ((rc = workspace_of("kv4_attention", workspace, workspace_bytes, need))) return rc;
   if (T == 0 || n == 0) return PH_OK;
   const Kv4AttnArgs a{q.base, o.base, reinterpret_cast<float*>(l.base), q.ld, o.ld, l.ld, static_cast<int>(T), n,
                       static_cast<int>(q_heads), window, slots, indptr, scale};

@@ -30,23 +30,32 @@ _PACK = struct.Struct("<Qiiqqqqq").pack     # PhTensor, as the C compiler lays i
 assert struct.calcsize("<Qiiqqqqq") == ctypes.sizeof(PhTensor)
 
 
-def _codes():
+_torch = None          # imported at the first call, as everywhere in this package
+_CODES = {}
+_get_device = _get_stream = None
+
+
+def _load_torch():
+    global _torch, _CODES, _get_device, _get_stream
     import torch
-    return {torch.float16: F16, torch.float32: F32, torch.int8: I8, torch.uint8: I8, torch.int32: I32}
+    _CODES = {torch.float16: F16, torch.float32: F32, torch.int8: I8, torch.uint8: I8, torch.int32: I32}
+    # The raw getters cost a tenth of the documented ones (which build a Stream object, and check each time that CUDA is
+    # up): much of a short call.  Where a torch lacks them the documented ones serve.
+    torch.cuda.init()
+    _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _get_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    _torch = torch
 
 
 def _device() -> int:
-    import torch
-    return torch.cuda.current_device()
+    if _torch is None:
+        _load_torch()
+    return _get_device()
 
 
 def _stream(stream, device: int) -> int:
-    """The stream's handle.  (The raw handle of the current one costs a tenth of what building a Stream object does, which
-    is much of a short call.)"""
     if stream is None:
-        import torch
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
+        return _get_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -59,10 +68,8 @@ def _on_device(t, name: str, device: int) -> None:
 
 def _desc(t, name: str, device: int) -> bytes:
     """A PhTensor, as bytes, of a rank-1/2 CUDA tensor of any element type these entry points know (no copy)."""
-    global _CODES
-    if _CODES is None:
-        _CODES = _codes()
-    _on_device(t, name, device)
+    if t.get_device() != device:
+        _on_device(t, name, device)
     code = _CODES.get(t.dtype)
     if code is None:
         raise PhobosError(PH_ERR_UNSUPPORTED, f"{name}: element type {t.dtype}")
@@ -74,9 +81,6 @@ def _desc(t, name: str, device: int) -> bytes:
     raise PhobosError(PH_ERR_INVALID, f"{name}: rank {len(size)}, expected 1 or 2")
 
 
-_CODES = None
-
-
 def byte_desc(t) -> PhTensor:
     """The descriptor of `launch` for a tensor that is not f16 or f32."""
     return PhTensor.from_buffer_copy(_desc(t, "tensor", _device()))
@@ -86,9 +90,9 @@ def _ints(t, name: str, device: int, n: int = 0):
     """Address of a contiguous int32 device tensor of at least n values (None stays None)."""
     if t is None:
         return None
-    _on_device(t, name, device)
-    import torch
-    if t.dtype is not torch.int32 or not t.is_contiguous():
+    if t.get_device() != device:
+        _on_device(t, name, device)
+    if t.dtype is not _torch.int32 or not t.is_contiguous():
         raise PhobosError(PH_ERR_INVALID, f"{name}: expected a contiguous int32 tensor")
     if t.numel() < n:
         raise PhobosError(PH_ERR_INVALID, f"{name}: {t.numel()} values, expected {n}")

@@ -156,7 +156,7 @@ def test_refusals(ph, dev):
     x, w, y = torch.randn(4, K, device=dev).half(), ph.q4_pack(code, scale, zero, G), torch.empty(4, N, device=dev)
     bad = [lambda: ph.gemv_q4(x.float(), w, y, G), lambda: ph.gemv_q4(x, w, y.to(torch.int32), G), lambda: ph.gemv_q4(x, w, y, 48),
            lambda: ph.gemv_q4(x[:, :200], w, y, G), lambda: ph.gemv_q4(x[:3], w, y, G), lambda: ph.gemv_q4(x, w[:-16], y, G),
-           lambda: ph.gemv_q4(x, w, y, 128) if False else ph.gemv_q4(x, w[4:], y, G), lambda: ph.gemv_q4(x[:, 1:257 - 64], w, y, G),
+           lambda: ph.gemv_q4(x, w[4:], y, G), lambda: ph.gemv_q4(x[:, 1:257 - 64], w, y, G),
            lambda: ph.gemv_q4(x, w, y.t(), G), lambda: ph.q4_pack(code, scale[:, :-1], zero, G), lambda: ph.q4_pack(code, scale, zero[:-1], G),
            lambda: ph.q4_pack(code.int(), scale, zero, G), lambda: ph.q4_pack(code, scale.float(), zero, G),
            lambda: ph.q4_pack(code, scale, zero, G, out=w[:100]), lambda: ph.gemv_q4(x.cpu(), w, y, G)]
