@@ -106,15 +106,14 @@ def lib() -> ctypes.CDLL:
             "phobos_flash_workspace_bytes": (sz, [i32, i64, i64, i64, i64]),
             "phobos_last_launch_clock": (c.c_int, [vp, c.POINTER(u64), c.POINTER(u64)]),
             "phobos_selftest_bounded_wait": (c.c_int, [u64, vp]),
-            # (descriptors of these calls are packed bytes: see serve.py)
             "phobos_q4_packed_bytes": (sz, [i64, i64, i32]),
-            "phobos_q4_pack": (c.c_int, [vp, vp, vp, i32, vp, vp]),
-            "phobos_gemv_q4": (c.c_int, [vp, vp, vp, f32, f32, i32, vp]),
+            "phobos_q4_pack": (c.c_int, [TP, TP, TP, i32, TP, vp]),
+            "phobos_gemv_q4": (c.c_int, [TP, TP, TP, f32, f32, i32, vp]),
             "phobos_kv4_page_bytes": (sz, [i32, i32, i32, i32]),
-            "phobos_kv4_append": (c.c_int, [vp, i32, vp, vp, vp, vp, i32, vp]),
-            "phobos_kv4_read": (c.c_int, [vp, i32, vp, vp, vp, vp, i32, vp]),
+            "phobos_kv4_append": (c.c_int, [vp, i32, TP, TP, vp, vp, i32, vp]),
+            "phobos_kv4_read": (c.c_int, [vp, i32, TP, TP, vp, vp, i32, vp]),
             "phobos_kv4_attention_workspace_bytes": (sz, [vp, i64, i32, i32]),
-            "phobos_kv4_attention": (c.c_int, [vp, i32, vp, vp, vp, f32, i32, vp, vp, i32, vp, sz, vp]),
+            "phobos_kv4_attention": (c.c_int, [vp, i32, TP, TP, TP, f32, i32, vp, vp, i32, vp, sz, vp]),
             "phobos_kv4_pages_workspace_bytes": (sz, [vp]),
             "phobos_kv4_extend": (c.c_int, [vp, vp, vp, i32, vp, vp, sz, vp]),
             "phobos_kv4_fork": (c.c_int, [vp, vp, vp, i32, i32, vp, vp, sz, vp]),

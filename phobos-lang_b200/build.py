@@ -8,6 +8,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -15,6 +16,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 LIB = HERE / "libphobos_leaf.so"
+BIND = HERE / "_bind.so"            # CPython module of serve.py's short calls
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_f32.cu", "flash.cu", "elementwise.cu", "kda.cu", "tmap.cu", "noalloc.cu", "selftest.cu",
            "gemv_q4.cu", "gemv_q4_tc.cu", "kv4_cache.cu", "kv4_attn.cu", "kv4_pages.cu", "serve_api.cu",
            "host.cpp", "executor.cpp", "source.cpp", "planner.cpp", "plan_api.cpp", "wire.cpp"]
@@ -38,7 +40,7 @@ def _deps_mtime() -> float:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     sources = [s for s in SOURCES if (CSRC / s).exists()]
-    if not force and LIB.exists() and LIB.stat().st_mtime >= _deps_mtime():
+    if not force and all(so.exists() and so.stat().st_mtime >= _deps_mtime() for so in (LIB, BIND)):
         return LIB
     OBJ.mkdir(exist_ok=True)
     nvcc = _nvcc()
@@ -67,6 +69,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     r = subprocess.run(link, capture_output=True, text=True, env=env)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    r = subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
+                        str(CSRC / "bind.cpp"), "-o", str(BIND)], capture_output=True, text=True, env=env)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
     return LIB
 
 

@@ -14,9 +14,9 @@ Calls enqueue on the current (or given) stream; index arrays are int32 device te
 from __future__ import annotations
 
 import ctypes
-import struct
+import importlib.util
 
-from . import (F16, F32, I8, I32, PH_ERR_INVALID, PH_ERR_UNSUPPORTED, PhobosError, PhTensor, check, lib)
+from . import (F16, F32, I8, I32, PH_ERR_INVALID, PH_ERR_UNSUPPORTED, LIB_PATH, PhobosError, PhTensor, _stream_ptr, check, lib)
 
 
 class PhKv4Cache(ctypes.Structure):
@@ -26,84 +26,57 @@ class PhKv4Cache(ctypes.Structure):
                 ("group", ctypes.c_int32), ("max_seqs", ctypes.c_int32), ("table_width", ctypes.c_int32)]
 
 
-_PACK = struct.Struct("<Qiiqqqqq").pack     # PhTensor, as the C compiler lays it out
-assert struct.calcsize("<Qiiqqqqq") == ctypes.sizeof(PhTensor)
+_bind = None           # the CPython module with the short calls (csrc/bind.cpp), loaded at the first call
 
 
-_torch = None          # imported at the first call, as everywhere in this package
-_CODES = {}
-_get_device = _get_stream = None
-
-
-def _load_torch():
-    global _torch, _CODES, _get_device, _get_stream
+def _load():
+    """Loads csrc/bind.cpp's module and gives it what it calls; raises if it has not been built (no fallback exists)."""
+    global _bind
+    path = LIB_PATH.parent / "_bind.so"
+    if not path.exists():
+        raise ImportError(f"{path} is missing: build it with `python phobos-lang_b200/build.py`")
     import torch
-    _CODES = {torch.float16: F16, torch.float32: F32, torch.int8: I8, torch.uint8: I8, torch.int32: I32}
-    # The raw getters cost a tenth of the documented ones (which build a Stream object, and check each time that CUDA is
-    # up): much of a short call.  Where a torch lacks them the documented ones serve.
     torch.cuda.init()
-    _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-    _get_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
-    _torch = torch
+    spec = importlib.util.spec_from_file_location("_bind", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    L = lib()
+    entries = tuple(ctypes.cast(getattr(L, "phobos_" + n), ctypes.c_void_p).value for n in
+                    ("gemv_q4", "kv4_append", "kv4_read", "kv4_attention", "kv4_extend", "kv4_fork", "kv4_free", "kv4_compact"))
+    # The raw getters cost a tenth of the documented ones, which build a Stream object and check each time that CUDA is up.
+    # Where a torch lacks them the documented ones serve.
+    device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    module.setup(entries, (torch.float16, torch.float32, torch.int8, torch.uint8, torch.int32), PhobosError, device, stream)
+    _bind = module
+    return module
 
 
 def _device() -> int:
-    if _torch is None:
-        _load_torch()
-    return _get_device()
-
-
-def _stream(stream, device: int) -> int:
-    if stream is None:
-        return _get_stream(device)
-    return stream if isinstance(stream, int) else stream.cuda_stream
+    import torch
+    return torch.cuda.current_device()
 
 
 def _on_device(t, name: str, device: int) -> None:
-    if t.get_device() != device:      # -1 for a CPU tensor
-        if not t.is_cuda:
-            raise PhobosError(PH_ERR_INVALID, f"{name} is not on a CUDA device")
+    if not t.is_cuda:
+        raise PhobosError(PH_ERR_INVALID, f"{name} is not on a CUDA device")
+    if t.device.index != device:
         raise PhobosError(PH_ERR_INVALID, f"{name} lives on cuda:{t.device.index} but the current device is cuda:{device}")
 
 
-def _desc(t, name: str, device: int) -> bytes:
-    """A PhTensor, as bytes, of a rank-1/2 CUDA tensor of any element type these entry points know (no copy)."""
-    if t.get_device() != device:
-        _on_device(t, name, device)
-    code = _CODES.get(t.dtype)
-    if code is None:
+def byte_desc(t, name: str = "tensor") -> PhTensor:
+    """PhTensor of a rank-1/2 CUDA tensor of any element type these entry points know (no copy)."""
+    import torch
+    _on_device(t, name, _device())
+    codes = {torch.float16: F16, torch.float32: F32, torch.int8: I8, torch.uint8: I8, torch.int32: I32}
+    if t.dtype not in codes:
         raise PhobosError(PH_ERR_UNSUPPORTED, f"{name}: element type {t.dtype}")
-    size, stride = t.shape, t.stride()
-    if len(size) == 2:
-        return _PACK(t.data_ptr(), code, 2, size[0], size[1], stride[0], stride[1], 0)
-    if len(size) == 1:
-        return _PACK(t.data_ptr(), code, 1, size[0], 0, stride[0], 0, 0)
-    raise PhobosError(PH_ERR_INVALID, f"{name}: rank {len(size)}, expected 1 or 2")
-
-
-def byte_desc(t) -> PhTensor:
-    """The descriptor of `launch` for a tensor that is not f16 or f32."""
-    return PhTensor.from_buffer_copy(_desc(t, "tensor", _device()))
-
-
-def _ints(t, name: str, device: int, n: int = 0):
-    """Address of a contiguous int32 device tensor of at least n values (None stays None)."""
-    if t is None:
-        return None
-    if t.get_device() != device:
-        _on_device(t, name, device)
-    if t.dtype is not _torch.int32 or not t.is_contiguous():
-        raise PhobosError(PH_ERR_INVALID, f"{name}: expected a contiguous int32 tensor")
-    if t.numel() < n:
-        raise PhobosError(PH_ERR_INVALID, f"{name}: {t.numel()} values, expected {n}")
-    return t.data_ptr()
-
-
-def _space(workspace, device: int):
-    if workspace is None:
-        return None, 0
-    _on_device(workspace, "workspace", device)
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if t.dim() not in (1, 2):
+        raise PhobosError(PH_ERR_INVALID, f"{name}: rank {t.dim()}, expected 1 or 2")
+    d = PhTensor(t.data_ptr(), codes[t.dtype], t.dim())
+    for i in range(t.dim()):
+        d.sizes[i], d.strides[i] = t.shape[i], t.stride(i)
+    return d
 
 
 # ---- 4-bit weights ----------------------------------------------------------------------------
@@ -117,18 +90,18 @@ def q4_pack(codes, scales, zeros, group: int, out=None, stream=None):
     if out is None:
         need = q4_packed_bytes(codes.shape[0], codes.shape[1], group)
         out = torch.empty(need, dtype=torch.int8, device=codes.device)
-    dev = _device()
-    z = _desc(zeros, "zeros", dev) if zeros is not None else None
-    check(lib().phobos_q4_pack(_desc(codes, "codes", dev), _desc(scales, "scales", dev), z, group, _desc(out, "packed", dev),
-                               _stream(stream, dev)))
+    c, s, o = byte_desc(codes, "codes"), byte_desc(scales, "scales"), byte_desc(out, "packed")
+    z = byte_desc(zeros, "zeros") if zeros is not None else None
+    check(lib().phobos_q4_pack(ctypes.byref(c), ctypes.byref(s), ctypes.byref(z) if z is not None else None, group, ctypes.byref(o),
+                               _stream_ptr(stream)))
     return out
 
 
 def gemv_q4(X, packed, Y, group: int, alpha: float = 1.0, beta: float = 0.0, stream=None) -> None:
     """Y[M,N] = alpha * X[M,K] W[N,K]^T + beta * Y, W = scale * (code - zero) in 4 bits; X f16, Y f16 or f32."""
-    dev = _device()
-    check(lib().phobos_gemv_q4(_desc(X, "X", dev), _desc(packed, "packed", dev), _desc(Y, "Y", dev), alpha, beta, group,
-                               _stream(stream, dev)))
+    rc = (_bind or _load()).gemv_q4(X, packed, Y, group, alpha, beta, stream)
+    if rc:
+        check(rc)
 
 
 # ---- the cache ------------------------------------------------------------------------------------
@@ -144,6 +117,10 @@ class Kv4Cache:
         dev = _device()
         for t, name in ((pages, "pages"), (refs, "refs"), (tables, "tables"), (lens, "lens")):
             _on_device(t, name, dev)
+        import torch
+        for t, name in ((refs, "refs"), (tables, "tables"), (lens, "lens")):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise PhobosError(PH_ERR_INVALID, f"{name}: expected a contiguous int32 tensor")
         need = kv4_page_bytes(kv_heads, head_dim, group, page_tokens)
         if need == 0:
             raise PhobosError(PH_ERR_UNSUPPORTED, f"kv4: {kv_heads} heads of {head_dim} dims in groups of {group}, pages of "
@@ -156,10 +133,11 @@ class Kv4Cache:
         self.pages, self.refs, self.tables, self.lens = pages, refs, tables, lens
         self.kv_heads, self.head_dim, self.group, self.page_tokens = kv_heads, head_dim, group, page_tokens
         pitch = pages.stride(0) if pages.shape[0] > 1 else 0
-        self.struct = PhKv4Cache(pages.data_ptr(), _ints(refs, "refs", dev), _ints(tables, "tables", dev), _ints(lens, "lens", dev), pitch,
+        self.struct = PhKv4Cache(pages.data_ptr(), refs.data_ptr(), tables.data_ptr(), lens.data_ptr(), pitch,
                                  pages.shape[0], pages.shape[1], page_tokens, kv_heads, head_dim, group, tables.shape[0],
                                  tables.shape[1])
-        self.address, self.device = ctypes.addressof(self.struct), dev
+        self.address = ctypes.addressof(self.struct)
+        self.handle = (self.address, dev)      # for csrc/bind.cpp
 
     @classmethod
     def create(cls, layers: int, n_pages: int, kv_heads: int, head_dim: int, group: int, page_tokens: int, max_seqs: int,
@@ -173,24 +151,18 @@ class Kv4Cache:
                    kv_heads=kv_heads, head_dim=head_dim, group=group, page_tokens=page_tokens)
 
 
-def _batch(cache: Kv4Cache, slots, indptr):
-    dev = _device()
-    if cache.device != dev:
-        raise PhobosError(PH_ERR_INVALID, f"the cache lives on cuda:{cache.device} but the current device is cuda:{dev}")
-    n = slots.numel()
-    return dev, _ints(slots, "slots", dev), _ints(indptr, "indptr", dev, n + 1), n
-
-
 def kv4_append(cache: Kv4Cache, layer: int, K, V, slots, indptr=None, stream=None) -> None:
     """Quantises rows K, V [T, kv_heads * head_dim] into the places of the sequences' last tokens (see kv4_extend)."""
-    dev, s, i, n = _batch(cache, slots, indptr)
-    check(lib().phobos_kv4_append(cache.address, layer, _desc(K, "K", dev), _desc(V, "V", dev), s, i, n, _stream(stream, dev)))
+    rc = (_bind or _load()).rows(0, cache.handle, layer, K, V, slots, indptr, stream)
+    if rc:
+        check(rc)
 
 
 def kv4_read(cache: Kv4Cache, layer: int, K, V, slots, indptr=None, stream=None) -> None:
     """The values of the sequences' last tokens into rows K, V: the inverse of kv4_append."""
-    dev, s, i, n = _batch(cache, slots, indptr)
-    check(lib().phobos_kv4_read(cache.address, layer, _desc(K, "K", dev), _desc(V, "V", dev), s, i, n, _stream(stream, dev)))
+    rc = (_bind or _load()).rows(1, cache.handle, layer, K, V, slots, indptr, stream)
+    if rc:
+        check(rc)
 
 
 def kv4_attention_workspace_bytes(cache: Kv4Cache, T: int, n: int, q_heads: int) -> int:
@@ -201,11 +173,9 @@ def kv4_attention(cache: Kv4Cache, layer: int, Q, O, scale: float, slots, indptr
                   stream=None) -> None:
     """O = softmax(scale q K^T) V over the cache; Q, O [T, q_heads * head_dim] f16.  The row of position p sees tokens
     j <= p (window > 0: only j > p - window); one that sees nothing gets zeros and lse -inf."""
-    dev, s, i, n = _batch(cache, slots, indptr)
-    l = _desc(lse, "lse", dev) if lse is not None else None
-    wp, wn = _space(workspace, dev)
-    check(lib().phobos_kv4_attention(cache.address, layer, _desc(Q, "Q", dev), _desc(O, "O", dev), l, scale, window, s, i, n, wp, wn,
-                                     _stream(stream, dev)))
+    rc = (_bind or _load()).attention(cache.handle, layer, Q, O, lse, scale, window, slots, indptr, workspace, stream)
+    if rc:
+        check(rc)
 
 
 def kv4_pages_workspace_bytes(cache: Kv4Cache) -> int:
@@ -215,28 +185,27 @@ def kv4_pages_workspace_bytes(cache: Kv4Cache) -> int:
 def kv4_extend(cache: Kv4Cache, slots, counts, shortfall, workspace=None, stream=None) -> None:
     """Room for counts[i] more tokens of slots[i], and the new lengths.  shortfall (int32 [1], device): 0 done, > 0 pages
     missing, -1 a wrong request; unless it is 0 nothing has changed and the rows must not be appended."""
-    dev, s, _, n = _batch(cache, slots, None)
-    wp, wn = _space(workspace, dev)
-    check(lib().phobos_kv4_extend(cache.address, s, _ints(counts, "counts", dev, n), n, _ints(shortfall, "shortfall", dev, 1), wp, wn,
-                                  _stream(stream, dev)))
+    rc = (_bind or _load()).extend(cache.handle, slots, counts, shortfall, workspace, stream)
+    if rc:
+        check(rc)
 
 
 def kv4_fork(cache: Kv4Cache, src, dst, shortfall, deep: bool = False, workspace=None, stream=None) -> None:
     """The empty sequences dst[i] continue from src[i], sharing its pages, or (deep) with copies of them."""
-    dev, s, _, n = _batch(cache, src, None)
-    wp, wn = _space(workspace, dev)
-    check(lib().phobos_kv4_fork(cache.address, s, _ints(dst, "dst", dev, n), n, int(deep), _ints(shortfall, "shortfall", dev, 1), wp, wn,
-                                _stream(stream, dev)))
+    rc = (_bind or _load()).fork(cache.handle, src, dst, int(deep), shortfall, workspace, stream)
+    if rc:
+        check(rc)
 
 
 def kv4_free(cache: Kv4Cache, slots, keep=None, stream=None) -> None:
     """Shortens slots[i] to keep[i] tokens (None: to none) and gives the pages behind them back."""
-    dev, s, _, n = _batch(cache, slots, None)
-    check(lib().phobos_kv4_free(cache.address, s, _ints(keep, "keep", dev, n), n, _stream(stream, dev)))
+    rc = (_bind or _load()).free(cache.handle, slots, keep, stream)
+    if rc:
+        check(rc)
 
 
 def kv4_compact(cache: Kv4Cache, live, workspace=None, stream=None) -> None:
     """Moves the pages in use to ids 0 .. live[0] - 1 in every layer."""
-    dev, _, _, _ = _batch(cache, live, None)
-    wp, wn = _space(workspace, dev)
-    check(lib().phobos_kv4_compact(cache.address, _ints(live, "live", dev, 1), wp, wn, _stream(stream, dev)))
+    rc = (_bind or _load()).compact(cache.handle, live, workspace, stream)
+    if rc:
+        check(rc)
