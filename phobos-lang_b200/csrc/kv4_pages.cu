@@ -42,6 +42,18 @@ __host__ inline Plan plan_of(const Kv4View& c, void* ws) {
   return p;
 }
 
+// The rows' arrays of a call stand in shared memory where they fit: a planning block reads back what it wrote three times,
+// and each time costs a trip to L2 otherwise.
+constexpr int PLAN_SHARED = 48 * 1024;
+__host__ inline int plan_shared(const Kv4View& c) { return c.max_seqs <= PLAN_SHARED / 12 ? c.max_seqs * 12 : 0; }
+__device__ __forceinline__ void use_shared(const Kv4View& c, Plan* p) {
+  extern __shared__ int rows_of_call[];
+  if (c.max_seqs > PLAN_SHARED / 12) return;
+  p->claim = rows_of_call;
+  p->fresh = rows_of_call + c.max_seqs;
+  p->last = rows_of_call + 2 * c.max_seqs;
+}
+
 // Exclusive prefix sum over the CTA, and the total; all threads call.
 __device__ __forceinline__ int block_scan(int v, int* total) {
   __shared__ int warp_sum[33];
@@ -129,6 +141,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_plan_kernel(Kv4View c, Pl
                                                                    int* shortfall) {
   pdl_wait();
   pdl_launch_dependents();
+  use_shared(c, &p);
   __shared__ int wrong, moves;
   if (threadIdx.x == 0) {
     wrong = 0;
@@ -214,6 +227,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Kv4View c, Plan
                                                                  int deep, int* shortfall) {
   pdl_wait();
   pdl_launch_dependents();
+  use_shared(c, &p);
   __shared__ int wrong;
   if (threadIdx.x == 0) {
     wrong = 0;
@@ -335,25 +349,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_plan_kernel(Kv4View c, P
   }
 }
 
-// Tables after a compaction: pages at L (= *live) and above have moved.
-__global__ void __launch_bounds__(MOVE_THREADS) remap_kernel(Kv4View c, Plan p, const int* live) {
+// Moves pages of every layer; the list and its length come from the plan.  An item is 16 KB of one page.  After a
+// compaction's plan (live not null) it also renames the pages at L = *live and above in the tables.
+__global__ void __launch_bounds__(MOVE_THREADS) move_kernel(Kv4View c, Plan p, const int* live) {
   pdl_wait();
   pdl_launch_dependents();
-  const int l = *live;
-  for (int slot = blockIdx.x; slot < c.max_seqs; slot += gridDim.x) {
-    const int used = min(pages_for(c, max(c.lens[slot], 0)), c.table_width);
-    int* row = c.tables + static_cast<long long>(slot) * c.table_width;
-    for (int k = threadIdx.x; k < used; k += MOVE_THREADS) {
-      const int page = row[k];
-      if (page >= l && page < c.n_pages) row[k] = p.pages[page];
+  const int* n_moves = p.n_moves;
+  const int2* moves = p.moves;
+  if (live) {
+    const int l = *live;
+    for (int slot = blockIdx.x; slot < c.max_seqs; slot += gridDim.x) {
+      const int used = min(pages_for(c, max(c.lens[slot], 0)), c.table_width);
+      int* row = c.tables + static_cast<long long>(slot) * c.table_width;
+      for (int k = threadIdx.x; k < used; k += MOVE_THREADS) {
+        const int page = row[k];
+        if (page >= l && page < c.n_pages) row[k] = p.pages[page];
+      }
     }
   }
-}
-
-// Moves pages of every layer; the list and its length come from the plan.  An item is 16 KB of one page.
-__global__ void __launch_bounds__(MOVE_THREADS) move_kernel(Kv4View c, const int* n_moves, const int2* moves) {
-  pdl_wait();
-  pdl_launch_dependents();
   constexpr int ITEM = 16384;
   const int chunks = static_cast<int>((c.page_bytes + ITEM - 1) / ITEM);
   const long long items = static_cast<long long>(*n_moves) * c.layers * chunks;
@@ -381,10 +394,12 @@ struct Launches {
   cudaStream_t stream;
   cudaError_t error = cudaSuccess;
   template <typename... KArgs, typename... Args>
-  void add(void (*kernel)(KArgs...), int blocks, int threads, Args... args) {
-    if (error == cudaSuccess) error = launch_with_pdl(kernel, dim3(blocks), dim3(threads), 0, stream, args...);
+  void add(void (*kernel)(KArgs...), int blocks, int threads, int shared, Args... args) {
+    if (error == cudaSuccess) error = launch_with_pdl(kernel, dim3(blocks), dim3(threads), shared, stream, args...);
   }
-  void move(const Kv4View& c, const Plan& p, int sm_count) { add(move_kernel, sm_count * 8, MOVE_THREADS, c, p.n_moves, p.moves); }
+  void move(const Kv4View& c, const Plan& p, int sm_count, const int* live = nullptr) {
+    add(move_kernel, sm_count * 8, MOVE_THREADS, 0, c, p, live);
+  }
   int done(const char** err) const {
     if (error == cudaSuccess) return 0;
     *err = cudaGetErrorString(error);
@@ -403,7 +418,7 @@ int launch_kv4_extend(const Kv4View& c, const int* slots, const int* counts, int
                       int sm_count, cudaStream_t stream, const char** err) {
   const Plan p = plan_of(c, workspace);
   Launches l{stream};
-  l.add(extend_plan_kernel, 1, PLAN_THREADS, c, p, slots, counts, n, shortfall);
+  l.add(extend_plan_kernel, 1, PLAN_THREADS, plan_shared(c), c, p, slots, counts, n, shortfall);
   l.move(c, p, sm_count);
   return l.done(err);
 }
@@ -412,23 +427,22 @@ int launch_kv4_fork(const Kv4View& c, const int* src, const int* dst, int n, int
                     int sm_count, cudaStream_t stream, const char** err) {
   const Plan p = plan_of(c, workspace);
   Launches l{stream};
-  l.add(fork_plan_kernel, 1, PLAN_THREADS, c, p, src, dst, n, deep, shortfall);
+  l.add(fork_plan_kernel, 1, PLAN_THREADS, plan_shared(c), c, p, src, dst, n, deep, shortfall);
   if (deep) l.move(c, p, sm_count);
   return l.done(err);
 }
 
 int launch_kv4_free(const Kv4View& c, const int* slots, const int* keep, int n, cudaStream_t stream, const char** err) {
   Launches l{stream};
-  l.add(free_kernel, n, MOVE_THREADS, c, slots, keep, n);
+  l.add(free_kernel, n, MOVE_THREADS, 0, c, slots, keep, n);
   return l.done(err);
 }
 
 int launch_kv4_compact(const Kv4View& c, int* live, void* workspace, int sm_count, cudaStream_t stream, const char** err) {
   const Plan p = plan_of(c, workspace);
   Launches l{stream};
-  l.add(compact_plan_kernel, 1, PLAN_THREADS, c, p, live);
-  l.move(c, p, sm_count);
-  l.add(remap_kernel, c.max_seqs < 4 * sm_count ? c.max_seqs : 4 * sm_count, MOVE_THREADS, c, p, live);
+  l.add(compact_plan_kernel, 1, PLAN_THREADS, 0, c, p, live);
+  l.move(c, p, sm_count, live);
   return l.done(err);
 }
 
