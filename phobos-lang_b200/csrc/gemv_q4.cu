@@ -14,6 +14,9 @@
 // that a lane's 16-byte reads (the B operand of two matrix steps) meet no bank twice.  The tiles of W are dealt out evenly
 // over a grid that fills the GPU: a CTA whose share is not a multiple of WR RT leaves some products idle, which costs
 // nothing as long as the bytes are what is waited for.
+// Measured: 1 x 28672 x 8192, G = 128: 28.2 us, 4.4 TB/s (23.4 us without the products: bound by instructions, 123 for a
+// block of 16 x 128, half of them masks and shifts); 1 x 4096 x 4096: 4.8 us back to back in a graph.  Four tiles a warp
+// (x read and summed once for all of them) took 31 us where two took 34, sixteen rows a CTA in every case 37.
 #include <atomic>
 #include <type_traits>
 

@@ -20,6 +20,9 @@
 // sequence.  A problem whose units lie in one piece is finished there; one that was cut leaves (m, l, o) of its parts in
 // the workspace for a second, small kernel.  Warps share nothing: each streams its units through a ring of its own in
 // shared memory with bulk copies (one per unit, 2176 bytes at D = G = 128) that it issues itself.
+// Measured: 64 sequences of 1..8192 tokens, 8 heads of 128, 291 MB: 62 us, 4.7 TB/s, bound by instructions (257 a unit, issued
+// in half of all slots by 12 warps to an SM).  Eight rows a problem where no more can be there, else sixteen: the widening of
+// the codes is then done once for both halves (64 query heads on 4, G = 32: 73 us against 90).
 #include <atomic>
 
 #include "kv4.cuh"
