@@ -33,7 +33,7 @@ namespace {
 
 constexpr int AT_WARPS = 4;
 constexpr int AT_START = 8;             // places for starting a problem
-constexpr int AT_PIECE = AT_START + 4;  // a piece is at least that long: one tile
+constexpr int AT_PIECE = 4;             // a piece is at least that long: one tile
 constexpr uint32_t EIGHT = 0x00080008u;  // 8 * 2^-24, as a low nibble's 8, two f16
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum : uint32_t { SITE_KV4_RING = 0x41 };
@@ -91,50 +91,37 @@ __device__ __forceinline__ int seq_problems(const AttnParams& p, const Kv4Rows& 
   return p.c.heads * (((r.end - r.begin) * p.rep + ROWS - 1) / ROWS);
 }
 
-// Length of the line.  A whole warp calls.
-template <int ROWS>
-__device__ long long line_length(const AttnParams& p) {
-  long long sum = 0;
-  for (int b = threadIdx.x & 31; b < p.a.n; b += 32) {
-    const Kv4Rows r = kv4_rows(p.c, p.a.slots, p.a.ind, b, p.a.T, p.status);
-    int begin;
-    sum += static_cast<long long>(seq_units(p, r, &begin) + AT_START) * seq_problems<ROWS>(p, r);
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  return sum;
+// a / b for b > 0; most numbers here fit 32 bits, and a 64-bit division takes a hundred instructions.
+__device__ __forceinline__ long long divide(long long a, int b) {
+  return (a >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
 }
 
-// Walks the sequences, 32 at a time, from `*b` (which stands at `*line`) to the one that holds place `at`.  A whole warp
-// calls; false behind the last.
+// 32 sequences, one to a lane, and where they stand on the line.
+struct Chunk {
+  int first;             // sequence of lane 0
+  Kv4Rows rows;
+  long long begin, end;  // the lane's places, counted from the chunk's
+};
 template <int ROWS>
-__device__ bool find_sequence(const AttnParams& p, long long at, int* b, long long* line) {
+__device__ void load_chunk(const AttnParams& p, int first, Chunk* c) {
   const int lane = threadIdx.x & 31;
-  long long done = *line;
-  for (int i0 = *b; i0 < p.a.n; i0 += 32) {
-    long long places = 0;
-    if (i0 + lane < p.a.n) {
-      const Kv4Rows r = kv4_rows(p.c, p.a.slots, p.a.ind, i0 + lane, p.a.T, p.status);
-      int begin;
-      places = static_cast<long long>(seq_units(p, r, &begin) + AT_START) * seq_problems<ROWS>(p, r);
-    }
-    long long sum = places;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const long long v = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += v;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, done + sum > at);
-    if (past) {
-      const int k = __ffs(past) - 1;
-      *b = i0 + k;
-      *line = done + __shfl_sync(0xffffffffu, sum - places, k);
-      return true;
-    }
-    done += __shfl_sync(0xffffffffu, sum, 31);
+  long long places = 0;
+  c->first = first;
+  if (first + lane < p.a.n) {
+    c->rows = kv4_rows(p.c, p.a.slots, p.a.ind, first + lane, p.a.T, p.status);
+    int begin;
+    places = static_cast<long long>(seq_units(p, c->rows, &begin) + AT_START) * seq_problems<ROWS>(p, c->rows);
   }
-  return false;
+  long long sum = places;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long v = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += v;
+  }
+  c->begin = sum - places;
+  c->end = sum;
 }
+__device__ __forceinline__ long long length_of(const Chunk& c) { return __shfl_sync(0xffffffffu, c.end, 31); }
 
 // Running state of 8 NT query rows in one warp: lane 4g + t keeps rows 8k + 2t and 8k + 2t + 1.  Sums of p and of
 // p * zero are the lane's own tokens' only, until the end.
@@ -354,8 +341,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  const long long line = line_length<ROWS>(p);
-  const long long piece = max((line + p.pieces - 1) / p.pieces, static_cast<long long>(AT_PIECE));
+  Chunk chunk;
+  load_chunk<ROWS>(p, 0, &chunk);
+  long long line = length_of(chunk);
+  if (p.a.n > 32) {
+    for (int i = 32; i < p.a.n; i += 32) {
+      load_chunk<ROWS>(p, i, &chunk);
+      line += length_of(chunk);
+    }
+    load_chunk<ROWS>(p, 0, &chunk);
+  }
+  const long long piece = max(divide(line + p.pieces - 1, p.pieces), static_cast<long long>(AT_PIECE));
   const int me = blockIdx.x * AT_WARPS + warp;  // this warp's piece
   long long at = piece * me;
   const long long stop = min(at + piece, line);
@@ -365,16 +361,28 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
   const float cq = p.a.scale * LOG2E, cs = cq * Q4_LO_UNIT;
   const int page_units = 1 << (p.c.page_shift - 4);
   uint32_t phase = 0;  // tiles this warp has taken from its ring so far
-  int seq = 0;
-  long long seq_at = 0;
-  while (at < stop && find_sequence<ROWS>(p, at, &seq, &seq_at)) {
+  long long chunk_at = 0;  // where the chunk stands on the line
+  while (at < stop) {
     // ---- the sequence at `at`, and its problems from there on --------------------------------------------------------------
-    const Kv4Rows rows = kv4_rows(p.c, p.a.slots, p.a.ind, seq, p.a.T, p.status);
+    const unsigned past = __ballot_sync(0xffffffffu, chunk_at + chunk.end > at);
+    if (past == 0) {
+      chunk_at += length_of(chunk);
+      if (chunk.first + 32 >= p.a.n) break;  // (not reached: the line ends with the last sequence)
+      load_chunk<ROWS>(p, chunk.first + 32, &chunk);
+      continue;
+    }
+    const int of = __ffs(past) - 1;
+    const long long seq_at = chunk_at + __shfl_sync(0xffffffffu, chunk.begin, of);
+    Kv4Rows rows;
+    rows.begin = __shfl_sync(0xffffffffu, chunk.rows.begin, of);
+    rows.end = __shfl_sync(0xffffffffu, chunk.rows.end, of);
+    rows.length = __shfl_sync(0xffffffffu, chunk.rows.length, of);
+    rows.slot = __shfl_sync(0xffffffffu, chunk.rows.slot, of);
     const int n_rows = (rows.end - rows.begin) * p.rep, first = rows.length - (rows.end - rows.begin);
     int u_begin;
     const int units = seq_units(p, rows, &u_begin), span = units + AT_START, problems = seq_problems<ROWS>(p, rows);
     const int tiles = problems / p.c.heads;
-    for (int index = static_cast<int>((at - seq_at) / span); index < problems && at < stop; index++) {
+    for (int index = static_cast<int>(divide(at - seq_at, span)); index < problems && at < stop; index++) {
       const int head = index / tiles, row0 = (index - head * tiles) * ROWS;
       const long long start = seq_at + static_cast<long long>(index) * span;  // of the problem, on the line
       const bool continued = at > start;
@@ -552,7 +560,7 @@ constexpr int JOIN_THREADS = 512;
 // b + gridDim.x, ... all at once, for most pieces end without a cut, and joins those that there are.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, int split) {
-  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, CHUNK = 256, FEW = 8;
+  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, CHUNK = JOIN_THREADS, FEW = 16;
   __shared__ float weight[CHUNK], top[JOIN_THREADS / 32], so[GROUPS][D], sl[JOIN_THREADS / 32];
   __shared__ int list[JOIN_THREADS], listed;
   if (threadIdx.x == 0) listed = 0;

@@ -117,7 +117,12 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p
   const int groups = D / p.c.G, unit_bytes = kv4_unit_bytes(D, p.c.G), page_units = 1 << (p.c.page_shift - 4);
   const bool value = (lane % (2 * W)) >= W;
   const int word = lane % W, grp = word * 8 / p.c.G;
-  for (int head = warp; head < p.c.heads; head += ROW_WARPS) {
+  // of a unit that is not whole every warp takes one batch of rows of one head, so that all can have some
+  constexpr int BATCHES = PASSES / AHEAD;
+  const int jobs = whole ? p.c.heads : p.c.heads * BATCHES;
+  for (int at = warp; at < jobs; at += ROW_WARPS) {
+    const int head = whole ? at : at / BATCHES, pass0 = whole ? 0 : at % BATCHES * AHEAD;
+    const int passes = whole ? PASSES : AHEAD;
     uint8_t* unit = p.c.pages + page * p.c.page_bytes +
                     (static_cast<long long>(head) * page_units + (job.unit & (page_units - 1))) * unit_bytes;
     uint8_t* to = whole ? image[warp] : unit;
@@ -128,9 +133,9 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p
       __syncwarp();
     }
     uint4 rows[AHEAD];
-#pragma unroll
-    for (int k = 0; k < PASSES; k++) {
-      const int r = k * AT_ONCE + lane / (2 * W);
+#pragma unroll 4
+    for (int k = 0; k < passes; k++) {
+      const int r = (pass0 + k) * AT_ONCE + lane / (2 * W);
       const bool live = r >= r0 && r < r1;
       if constexpr (!READ) {
         if (k % AHEAD == 0) {

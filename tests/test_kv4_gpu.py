@@ -235,7 +235,7 @@ def test_chunks_of_queries(ph, dev, D, G, rep, page):
 
 
 @pytest.mark.parametrize("D,G,Hkv,rep,lens", [(128, 128, 1, 8, [20000, 3, 7000]), (64, 64, 2, 4, [33000]), (128, 32, 8, 1, [5000, 4999, 1, 2500, 16, 1000, 777, 64, 65]),
-                                              (128, 64, 1, 16, [9000, 100])])
+                                              (128, 64, 1, 16, [9000, 100]), (64, 64, 1, 1, [120000])])
 def test_long_and_uneven_sequences(ph, dev, D, G, Hkv, rep, lens):
     s = Setup(ph, dev, lens, Hkv, D, G, 64, seed=6)
     check(s, [1] * len(lens), rep)
