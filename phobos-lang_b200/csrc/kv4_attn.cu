@@ -362,13 +362,16 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
   const int page_units = 1 << (p.c.page_shift - 4);
   uint32_t phase = 0;  // tiles this warp has taken from its ring so far
   long long chunk_at = 0;  // where the chunk stands on the line
+  int next_chunk = -1;     // a chunk's registers are not held while a sequence is worked on
   while (at < stop) {
     // ---- the sequence at `at`, and its problems from there on --------------------------------------------------------------
+    if (next_chunk >= 0) load_chunk<ROWS>(p, next_chunk, &chunk);
+    next_chunk = chunk.first;
     const unsigned past = __ballot_sync(0xffffffffu, chunk_at + chunk.end > at);
     if (past == 0) {
       chunk_at += length_of(chunk);
-      if (chunk.first + 32 >= p.a.n) break;  // (not reached: the line ends with the last sequence)
-      load_chunk<ROWS>(p, chunk.first + 32, &chunk);
+      next_chunk += 32;
+      if (next_chunk >= p.a.n) break;  // (not reached: the line ends with the last sequence)
       continue;
     }
     const int of = __ffs(past) - 1;
@@ -556,12 +559,16 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
 
 constexpr int JOIN_THREADS = 512;
 
-// Joins the parts of problems that were cut.  An item is every `split`-th row of one problem; CTA b looks at items b,
-// b + gridDim.x, ... all at once, for most pieces end without a cut, and joins those that there are.
+// Joins the parts of problems that were cut.  An item is one row of a problem; CTA b looks at items b, b + gridDim.x, ... all
+// at once, for most pieces end without a cut, and joins those that there are: rows of up to JOIN_WARP parts a warp each, all
+// warps at the same time (no barrier in it), then the longer ones with the whole block.  (With a block to every row the 96
+// problems of 12 sequences of 1635 tokens, a dozen parts each, took 27 us to join.)
+constexpr int JOIN_WARP = 32;
+
 template <int D, int ROWS>
-__global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, int split) {
-  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, CHUNK = JOIN_THREADS, FEW = 16;
-  __shared__ float weight[CHUNK], top[JOIN_THREADS / 32], so[GROUPS][D], sl[JOIN_THREADS / 32];
+__global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, int rows) {
+  constexpr int PART = ROWS * (D + 2), GROUPS = JOIN_THREADS / D, WARPS = JOIN_THREADS / 32, DIMS = D / 32;
+  __shared__ float weight[JOIN_THREADS], top[WARPS], so[GROUPS][D], sl[WARPS];
   __shared__ int list[JOIN_THREADS], listed;
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
@@ -569,73 +576,101 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, in
   {
     // (the launch sees to it that a CTA has at most JOIN_THREADS items)
     const int item = blockIdx.x + threadIdx.x * gridDim.x;
-    if (item < p.pieces * split) {
-      const Cut& c = p.cuts[item / split];
-      if (c.parts > 0 && item % split < c.n_rows) list[atomicAdd(&listed, 1)] = item;
+    if (item < p.pieces * rows) {
+      const Cut& c = p.cuts[item / rows];
+      if (c.parts > 0 && item % rows < c.n_rows) list[atomicAdd(&listed, 1)] = item;
     }
   }
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x % D, group = threadIdx.x / D;
-  for (int at = 0; at < listed; at++) {
-    const Cut cut = p.cuts[list[at] / split];
-    const int n = cut.parts, row_begin = list[at] % split, row_step = split;
-    auto part_of = [&](int i) { return p.part + static_cast<long long>(i == 0 ? cut.first : cut.next + 2 * (i - 1)) * PART; };
-  auto write = [&](int r, int d, float m, float l, float o) {
-    const int row = cut.row0 + r, token = row / p.rep, h = cut.head * p.rep + row - token * p.rep;
-    const long long out = cut.row_begin + token;
-    static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
-    if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto part_of = [&](const Cut& cut, int i) {
+    return p.part + static_cast<long long>(i == 0 ? cut.first : cut.next + 2 * (i - 1)) * PART;
   };
-  if (n <= FEW) {  // every thread on its own
-    for (int r = row_begin + group * row_step; r < cut.n_rows; r += row_step * GROUPS) {
-      float mi[FEW], li[FEW], v[FEW], m = -INFINITY, l = 0.0f, o = 0.0f;
-#pragma unroll
-      for (int i = 0; i < FEW; i++) {
-        mi[i] = -INFINITY;
-        li[i] = v[i] = 0.0f;
-        if (i < n) {
-          const float* part = part_of(i);
-          mi[i] = part[ROWS * D + r];
-          li[i] = part[ROWS * D + ROWS + r];
-          v[i] = part[r * D + d];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < FEW; i++) m = fmaxf(m, mi[i]);
-#pragma unroll
-      for (int i = 0; i < FEW; i++) {
-        if (li[i] == 0.0f) continue;
-        const float f = exp2_approx(mi[i] - m);
-        l = fmaf(li[i], f, l);
-        o = fmaf(v[i], f, o);
-      }
-      write(r, d, m, l, o);
+  auto place = [&](const Cut& cut, int r, long long* out, int* h) {
+    const int row = cut.row0 + r, token = row / p.rep;
+    *out = cut.row_begin + token;
+    *h = cut.head * p.rep + row - token * p.rep;
+  };
+  bool longer = false;
+  for (int at = warp; at < listed; at += WARPS) {
+    const Cut cut = p.cuts[list[at] / rows];
+    const int n = cut.parts, r = list[at] % rows;
+    if (n > JOIN_WARP) {
+      longer = true;
+      continue;
     }
-    continue;
+    constexpr int AHEAD = 8;  // parts whose o is on its way while the weights are found
+    float v[AHEAD][DIMS];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; k++)
+        if (k0 + k < n) {
+          const float* from = part_of(cut, k0 + k) + r * D + lane * DIMS;
+#pragma unroll
+          for (int d = 0; d < DIMS; d++) v[k][d] = from[d];
+        }
+    };
+    fetch(0);
+    float mi = -INFINITY, l = 0.0f;
+    if (lane < n) {
+      const float* part = part_of(cut, lane);
+      mi = part[ROWS * D + r];
+      l = part[ROWS * D + ROWS + r];
+    }
+    float m = mi, o[DIMS] = {};
+#pragma unroll
+    for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const float f = l == 0.0f ? 0.0f : exp2_approx(mi - m);  // (the weight of a part that saw nothing)
+    l = l == 0.0f ? 0.0f : l * f;
+    for (int k0 = 0; k0 < n; k0 += AHEAD) {
+      if (k0 > 0) fetch(k0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; k++) {
+        const float fk = __shfl_sync(0xffffffffu, f, k0 + k);
+        if (k0 + k < n)
+#pragma unroll
+          for (int d = 0; d < DIMS; d++) o[d] = fmaf(v[k][d], fk, o[d]);
+      }
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k /= 2) l += __shfl_xor_sync(0xffffffffu, l, k);
+    long long out;
+    int h;
+    place(cut, r, &out, &h);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    __half* to = static_cast<__half*>(p.a.O) + out * p.a.ldo + h * D + lane * DIMS;
+#pragma unroll
+    for (int d = 0; d < DIMS; d += 2) *reinterpret_cast<__half2*>(to + d) = __floats2half2_rn(o[d] * inv, o[d + 1] * inv);
+    if (lane == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
   }
-  for (int r = row_begin; r < cut.n_rows; r += row_step) {
+  if (!__syncthreads_or(longer)) return;
+  const int d = threadIdx.x % D, group = threadIdx.x / D;
+  for (int at = 0; at < listed; at++) {
+    const Cut cut = p.cuts[list[at] / rows];
+    const int n = cut.parts, r = list[at] % rows;
+    if (n <= JOIN_WARP) continue;
     // the largest maximum, then every part's weight
     float m = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += JOIN_THREADS) m = fmaxf(m, part_of(i)[ROWS * D + r]);
+    for (int i = threadIdx.x; i < n; i += JOIN_THREADS) m = fmaxf(m, part_of(cut, i)[ROWS * D + r]);
 #pragma unroll
     for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     if (lane == 0) top[warp] = m;
     __syncthreads();
-    for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, top[w]);
+    for (int w = 0; w < WARPS; w++) m = fmaxf(m, top[w]);
     float l = 0.0f, o = 0.0f;
-    for (int i0 = 0; i0 < n; i0 += CHUNK) {
+    for (int i0 = 0; i0 < n; i0 += JOIN_THREADS) {
       const int i = i0 + threadIdx.x;
       if (i < n) {
-        const float* part = part_of(i);
+        const float* part = part_of(cut, i);
         const float mi = part[ROWS * D + r], li = part[ROWS * D + ROWS + r];
-        const float f = li == 0.0f ? 0.0f : exp2_approx(mi - m);  // (the weight of a part that saw nothing)
+        const float f = li == 0.0f ? 0.0f : exp2_approx(mi - m);
         weight[threadIdx.x] = f;
         if (li != 0.0f) l = fmaf(li, f, l);
       }
       __syncthreads();
-      const int end = min(n - i0, CHUNK);
+      const int end = min(n - i0, JOIN_THREADS);
 #pragma unroll 8
-      for (int k = group; k < end; k += GROUPS) o = fmaf(part_of(i0 + k)[r * D + d], weight[k], o);
+      for (int k = group; k < end; k += GROUPS) o = fmaf(part_of(cut, i0 + k)[r * D + d], weight[k], o);
       __syncthreads();
     }
 #pragma unroll
@@ -645,12 +680,15 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, in
     __syncthreads();
     if (group == 0) {
       l = o = 0.0f;
-      for (int w = 0; w < JOIN_THREADS / 32; w++) l += sl[w];
+      for (int w = 0; w < WARPS; w++) l += sl[w];
       for (int k = 0; k < GROUPS; k++) o += so[k][d];
-      write(r, d, m, l, o);
+      long long out;
+      int h;
+      place(cut, r, &out, &h);
+      static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
+      if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
     }
     __syncthreads();
-  }
   }
 }
 
@@ -691,11 +729,9 @@ cudaError_t launch_attn(AttnParams& p, int most_rows, int sm_count, cudaStream_t
   p.pieces = ctas * AT_WARPS;
   e = launch_with_pdl(kv4_attn_kernel<D, NG, NT, UN, STAGES>, dim3(ctas), dim3(AT_WARPS * 32), S::SMEM, stream, p);
   if (e != cudaSuccess) return e;
-  // few problems leave many parts each: an item a row; many leave few: an item as many rows as a CTA joins at a time
-  const int rows = min(most_rows, S::ROWS), split = problems <= sm_count ? rows : (rows + JOIN_THREADS / D - 1) / (JOIN_THREADS / D);
-  const int join_ctas = min(p.pieces * split, 4 * sm_count);
+  const int rows = min(most_rows, S::ROWS), join_ctas = min(p.pieces * rows, 4 * sm_count);
   static_assert(AT_MOST_PER_SM * AT_WARPS * S::ROWS <= 4 * JOIN_THREADS, "a CTA's items of the joining kernel");
-  return launch_with_pdl(kv4_join_kernel<D, S::ROWS>, dim3(join_ctas), dim3(JOIN_THREADS), 0, stream, p, split);
+  return launch_with_pdl(kv4_join_kernel<D, S::ROWS>, dim3(join_ctas), dim3(JOIN_THREADS), 0, stream, p, rows);
 }
 
 template <int D, int NG>
