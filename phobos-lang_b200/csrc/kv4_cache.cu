@@ -118,10 +118,10 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p
   const bool value = (lane % (2 * W)) >= W;
   const int word = lane % W, grp = word * 8 / p.c.G;
   // of a unit that is not whole every warp takes one batch of rows of one head, so that all can have some
-  constexpr int BATCHES = PASSES / AHEAD;
-  const int jobs = whole ? p.c.heads : p.c.heads * BATCHES;
+  constexpr int BATCH = AHEAD * AT_ONCE;
+  const int batch0 = r0 / BATCH, batches = whole ? 1 : (r1 - 1) / BATCH - batch0 + 1, jobs = p.c.heads * batches;
   for (int at = warp; at < jobs; at += ROW_WARPS) {
-    const int head = whole ? at : at / BATCHES, pass0 = whole ? 0 : at % BATCHES * AHEAD;
+    const int head = at / batches, pass0 = whole ? 0 : (batch0 + at % batches) * AHEAD;
     const int passes = whole ? PASSES : AHEAD;
     uint8_t* unit = p.c.pages + page * p.c.page_bytes +
                     (static_cast<long long>(head) * page_units + (job.unit & (page_units - 1))) * unit_bytes;
