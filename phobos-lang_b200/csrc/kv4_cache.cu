@@ -22,6 +22,7 @@ struct RowParams {
   const int* ind;
   int T, n;
   uint32_t* status;
+  bool images;  // whole units through shared memory
 };
 
 constexpr int ROW_WARPS = 8;
@@ -100,8 +101,9 @@ __device__ bool find_job(const RowParams& p, int at, Job* job) {
 }
 
 // One CTA: a unit of one sequence; each warp takes heads in turn.  D / 8 lanes work on a row's key and D / 8 on its value,
-// eight dims each, in as many rows at once as a warp holds.  A unit whose sixteen tokens are all there goes through shared
-// memory and is read or written in one piece of 16-byte words; of any other one only the rows' own bytes are touched.
+// eight dims each, in as many rows at once as a warp holds.  Where there are many, a unit whose sixteen tokens are all there
+// goes through shared memory, one head to a warp, and is read or written in one piece of 16-byte words; of any other one only
+// the rows' own bytes are touched, and its rows are shared out over the warps (350 rows of 4 heads: 12 us in whole units).
 template <int D, bool READ>
 __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p) {
   constexpr int W = D / 8, AT_ONCE = 32 / (2 * W), PASSES = KV4_UNIT / AT_ONCE, AHEAD = 4;
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = job.rows.end - job.rows.begin, first = job.rows.length - n;
   const int r0 = max(first - job.unit * 16, 0), r1 = min(job.rows.length - job.unit * 16, 16);  // its tokens r0 .. r1 - 1 are rows
-  const bool whole = r0 == 0 && r1 == 16;
+  const bool whole = r0 == 0 && r1 == 16 && p.images;
   const int page = job.unit >= 0 ? kv4_page(p.c, job.rows.slot, job.unit * 16, p.status) : -1;
   const int groups = D / p.c.G, unit_bytes = kv4_unit_bytes(D, p.c.G), page_units = 1 << (p.c.page_shift - 4);
   const bool value = (lane % (2 * W)) >= W;
@@ -236,13 +238,15 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 3) kv4_rows_kernel(RowParams p
 }
 
 template <bool READ>
-int launch_rows(const RowParams& p, cudaStream_t stream, const char** err) {
+int launch_rows(const RowParams& rows, cudaStream_t stream, const char** err) {
   // an upper bound on the units that the rows stand in: a sequence's first and last may be partly theirs
-  const long long jobs = p.ind ? static_cast<long long>(p.T) / KV4_UNIT + 2LL * p.n : p.n;
+  const long long jobs = rows.ind ? static_cast<long long>(rows.T) / KV4_UNIT + 2LL * rows.n : rows.n;
   if (jobs > 0x7fffffffLL) {
     *err = "kv4: too many rows";
     return -2;
   }
+  RowParams p = rows;
+  p.images = p.T >= 4096;  // 256 units, enough CTAs to fill the GPU
   const cudaError_t e = launch_with_pdl(p.c.D == 128 ? kv4_rows_kernel<128, READ> : kv4_rows_kernel<64, READ>, dim3(static_cast<unsigned>(jobs)),
                                         dim3(ROW_WARPS * 32), 0, stream, p);
   if (e == cudaSuccess) return 0;
@@ -254,13 +258,13 @@ int launch_rows(const RowParams& p, cudaStream_t stream, const char** err) {
 
 int launch_kv4_append(const Kv4View& c, const void* K, long long ldk, const void* V, long long ldv, int T, const int* slots,
                       const int* ind, int n, uint32_t* status, cudaStream_t stream, const char** err) {
-  const RowParams p{c, static_cast<const __half*>(K), static_cast<const __half*>(V), nullptr, nullptr, ldk, ldv, slots, ind, T, n, status};
+  const RowParams p{c, static_cast<const __half*>(K), static_cast<const __half*>(V), nullptr, nullptr, ldk, ldv, slots, ind, T, n, status, false};
   return launch_rows<false>(p, stream, err);
 }
 
 int launch_kv4_read(const Kv4View& c, void* K, long long ldk, void* V, long long ldv, int T, const int* slots, const int* ind,
                     int n, uint32_t* status, cudaStream_t stream, const char** err) {
-  const RowParams p{c, nullptr, nullptr, static_cast<__half*>(K), static_cast<__half*>(V), ldk, ldv, slots, ind, T, n, status};
+  const RowParams p{c, nullptr, nullptr, static_cast<__half*>(K), static_cast<__half*>(V), ldk, ldv, slots, ind, T, n, status, false};
   return launch_rows<true>(p, stream, err);
 }
 

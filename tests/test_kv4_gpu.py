@@ -162,6 +162,24 @@ def test_append_then_read_gives_the_quantised_values(ph, dev, D, G, page):
     assert ph.device_status() == 0 and T == s.ind[-1]
 
 
+def test_many_rows_at_once(ph, dev):
+    """Enough rows that whole units go through shared memory; ends of sequences that do not end a unit among them."""
+    import torch
+    for D, G in ((128, 32), (64, 64)):
+        s = Setup(ph, dev, [3000, 1, 1200, 17], 3, D, G, 64, seed=G)
+        ind = torch.tensor(s.ind, dtype=torch.int32, device=dev)
+        k, v = torch.full_like(s.k, 9.0), torch.full_like(s.v, 9.0)
+        ph.kv4_read(s.cache, 0, k, v, s.slots, ind)
+        for got, x in ((k, s.k), (v, s.v)):
+            want = value(x.unflatten(1, (3, D)), G).flatten(1)
+            assert bool(((got.double() - want).abs() <= 2.0 ** -11 * want.abs() * 1.001 + 2.0 ** -23).all())
+        small = torch.empty_like(s.k[:17]), torch.empty_like(s.v[:17])
+        ph.kv4_read(s.cache, 0, *small, s.slots[3:], torch.tensor([0, 17], dtype=torch.int32, device=dev))
+        assert torch.equal(small[0], k[-17:]) and torch.equal(small[1], v[-17:])
+        check(s, [1, 1, 1, 1], 2)
+    assert ph.device_status() == 0
+
+
 @pytest.mark.parametrize("D,G", [(64, 32), (128, 128)])
 def test_page_layout_is_the_documented_one(ph, dev, D, G):
     """The unit layout at the top of csrc/kv4.cuh, byte by byte; bytes of tokens that were not written stay."""
