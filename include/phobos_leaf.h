@@ -261,7 +261,7 @@ PH_API int phobos_kv4_read(const PhKv4Cache *cache, int32_t layer, const PhTenso
  * (head h reads key/value head h / (q_heads / kv_heads)).  The row of position p sees tokens j <= p, and with
  * window > 0 only j > p - window.  A row that sees nothing gets zeros.  lse, [T, q_heads] f32 or NULL: the natural
  * logarithm of the sum of exp(scale * q k), -inf for a row that sees nothing.  The workspace (256-byte aligned,
- * phobos_kv4_attention_workspace_bytes; its contents need not be kept) joins what several CTAs found of one sequence;
+ * phobos_kv4_attention_workspace_bytes; its contents need not be kept) holds what is found of one sequence in several places;
  * calls that share one must not overlap on the GPU. */
 PH_API size_t phobos_kv4_attention_workspace_bytes(const PhKv4Cache *cache, int64_t T, int32_t n, int32_t q_heads);
 PH_API int phobos_kv4_attention(const PhKv4Cache *cache, int32_t layer, const PhTensor *Q, const PhTensor *O,

@@ -104,11 +104,11 @@ bool describe(PyObject* t, const char* name, const Call& c, PhTensor* d) {
   return ok;
 }
 
-// Address and length of a contiguous int32 tensor of at least n values; None is a null address.
+// Address of a contiguous int32 tensor of at least n values, and its length where that is asked for; None is a null
+// address, but refused where the length counts.
 bool integers(PyObject* t, const char* name, const Call& c, long long n, int32_t** at, long long* count = nullptr) {
   *at = nullptr;
-  if (count) *count = 0;
-  if (t == Py_None) return true;
+  if (t == Py_None) return count == nullptr || refuse(PH_ERR_INVALID, "%s: expected a contiguous int32 tensor", name);
   if (!on_device(t, name, c)) return false;
   PyObject* type = PyObject_GetAttr(t, s_dtype);
   if (!type) return false;

@@ -56,12 +56,6 @@ struct GemvShape {
   static_assert(X_PITCH % 128 == 64 && W_BYTES % 64 == 0, "shared memory layout");
 };
 
-__device__ __forceinline__ void gemv_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // CTA (x, y): its share of the tiles of W, rows 8y .. 8y + 7 of X.
 template <int RT, int WR, int GS>
 __global__ void __launch_bounds__(GV_THREADS, GV_PER_SM) gemv_q4_kernel(GemvParams p) {
@@ -104,10 +98,10 @@ __global__ void __launch_bounds__(GV_THREADS, GV_PER_SM) gemv_q4_kernel(GemvPara
         if (lane == 0) mbar_arrive_expect_tx(full + st, n_tiles * w_each + n_m * x_each);
         __syncwarp();
         if (lane < n_tiles)
-          gemv_bulk_load(stage + x_bytes + lane * S::WK * S::BLOCK, p.W + (static_cast<long long>(tile0 + lane) * p.kblocks + kb) * S::BLOCK,
+          bulk_load(stage + x_bytes + lane * S::WK * S::BLOCK, p.W + (static_cast<long long>(tile0 + lane) * p.kblocks + kb) * S::BLOCK,
                          w_each, full + st);
         else if (lane - n_tiles < n_m)
-          gemv_bulk_load(stage + (lane - n_tiles) * S::X_PITCH, p.X + (m0 + lane - n_tiles) * p.ldx + kb * 128, x_each, full + st);
+          bulk_load(stage + (lane - n_tiles) * S::X_PITCH, p.X + (m0 + lane - n_tiles) * p.ldx + kb * 128, x_each, full + st);
         if (++st == p.stages) {
           st = 0;
           parity ^= 1;
@@ -327,12 +321,9 @@ cudaError_t launch_group(GemvParams& p, int sm_count, cudaStream_t stream) {
 
 int launch_gemv_q4(const void* X, long long ldx, const void* W, void* Y, long long ldy, int out_f32, int M, int N, int K,
                    int group, float alpha, float beta, int sm_count, uint32_t* status, cudaStream_t stream, const char** err) {
-  if (M > 8 && gemv_q4_tc_is_faster(M, N, K, group, sm_count))
+  // (more than 8 * 65535 rows of X are more than this kernel's grid holds)
+  if (M > 8 && (M > 8 * 65535 || gemv_q4_tc_is_faster(M, N, K, group, sm_count)))
     return launch_gemv_q4_tc(X, ldx, W, Y, ldy, out_f32, M, N, K, group, alpha, beta, sm_count, status, stream, err);
-  if (M > 8 * 65535) {
-    *err = "gemv_q4: too many rows of X";
-    return -2;
-  }
   GemvParams p{static_cast<const __half*>(X), static_cast<const uint8_t*>(W), Y, ldx, ldy, M, N, K, (K + 127) / 128,
                (N + 15) / 16, 0, 0, alpha, beta, out_f32, status};
   const cudaError_t e = group == 128  ? launch_group<8>(p, sm_count, stream)

@@ -63,12 +63,6 @@ struct TcGemvShape {
   static_assert(STAGES >= 3 && RED <= STAGES * STAGE && QT_A_SLOTS * QT_A_COLS + QT_D_SLOTS * NC <= QT_TMEM, "shape");
 };
 
-__device__ __forceinline__ void tc_gemv_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -163,7 +157,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
       if (lane == 0) mbar_arrive_expect_tx(full + s.slot, n_kb * (2 * S::X_BOX + n_tiles * S::BLOCK));
       __syncwarp();
       if (lane < n_tiles)
-        tc_gemv_bulk_load(stage + S::X_BYTES + lane * S::PITCH, p.W + (static_cast<long long>(tile0 + lane) * p.kblocks + kb) * S::BLOCK,
+        bulk_load(stage + S::X_BYTES + lane * S::PITCH, p.W + (static_cast<long long>(tile0 + lane) * p.kblocks + kb) * S::BLOCK,
                           n_kb * S::BLOCK, full + s.slot);
       else if (lane >= 16 && lane < 16 + 2 * n_kb)
         tma_load_2d(stage + (lane - 16) * S::X_BOX, &x_map, full + s.slot, kb * 128 + (lane - 16) * 64, m0);

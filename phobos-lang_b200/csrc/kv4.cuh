@@ -55,21 +55,4 @@ __device__ __forceinline__ int kv4_page(const Kv4View& c, int slot, int pos, uin
   return -1;
 }
 
-// The sequence whose rows hold `row`, found by the whole warp: the largest b with ind[b] <= row, as ind ascends.
-// Each pass looks at 32 places of what is left.
-__device__ __forceinline__ int kv4_find(const int* ind, int n, int row) {
-  if (!ind) return row;
-  const int lane = threadIdx.x & 31;
-  int lo = 0, len = n;  // ind[lo] <= row is taken for granted (ind[0] = 0)
-  while (len > 1) {
-    const int step = (len + 31) / 32;
-    const int at = lo + lane * step;
-    const unsigned le = __ballot_sync(0xffffffffu, at < lo + len && ind[at] <= row);
-    const int k = le ? 31 - __clz(le) : 0;
-    len = min(step, len - k * step);
-    lo += k * step;
-  }
-  return lo;
-}
-
 }  // namespace ph

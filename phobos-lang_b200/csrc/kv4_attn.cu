@@ -46,12 +46,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2^n for -126 <= n <= 127
 __device__ __forceinline__ float pow2i(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* at) {
   if constexpr (N == 4) {

@@ -45,7 +45,7 @@ __host__ inline Plan plan_of(const Kv4View& c, void* ws) {
 
 // The rows' arrays of a call stand in shared memory where they fit: a planning block reads back what it wrote three times,
 // and each time costs a trip to L2 otherwise.
-constexpr int PLAN_SHARED = 48 * 1024;
+constexpr int PLAN_SHARED = 40 * 1024;  // (with what the kernels have besides, within the 48 KB that need no asking)
 __host__ inline int plan_shared(const Kv4View& c) { return c.max_seqs <= PLAN_SHARED / 12 ? c.max_seqs * 12 : 0; }
 __device__ __forceinline__ void use_shared(const Kv4View& c, Plan* p) {
   extern __shared__ int rows_of_call[];

@@ -466,7 +466,8 @@ def test_refusals(ph, dev):
            lambda: att(window=-1), lambda: att(slots=s.slots.long()), lambda: att(slots=torch.zeros(2, dtype=torch.int32, device=dev)),
            lambda: att(lse=torch.empty(1, 3, device=dev)), lambda: att(lse=torch.empty(1, 4, device=dev).half()),
            lambda: att(ind=torch.zeros(1, dtype=torch.int32, device=dev)), lambda: att(q=torch.randn(1, 264, device=dev).half()[:, 4:260]),
-           lambda: att(ws=None), lambda: att(ws=ws[:need - 1]), lambda: att(ws=ws[8:]),
+           lambda: att(ws=None), lambda: ph.kv4_append(s.cache, 0, kv, kv, None), lambda: ph.kv4_append(s.cache, 0, kv.cpu(), kv, s.slots),
+           lambda: ph.kv4_append(s.cache, 0, kv.double(), kv, s.slots), lambda: ph.kv4_append(s.cache, 0, kv[0], kv[0], s.slots), lambda: att(ws=ws[:need - 1]), lambda: att(ws=ws[8:]),
            lambda: ph.kv4_append(s.cache, 0, kv, kv[:, :64], s.slots), lambda: ph.kv4_append(s.cache, 0, kv.float(), kv.float(), s.slots),
            lambda: ph.kv4_append(s.cache, 3, kv, kv, s.slots), lambda: ph.kv4_read(s.cache, 0, kv[:0], kv, s.slots),
            lambda: ph.Kv4Cache.create(1, 4, 2, 96, 32, 16, 2, 4), lambda: ph.Kv4Cache.create(1, 4, 2, 64, 128, 16, 2, 4),

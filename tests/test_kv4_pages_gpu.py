@@ -242,6 +242,19 @@ def test_many_sequences_and_pages(ph, dev):
     b.compact()
 
 
+@pytest.mark.parametrize("seqs", [1, 3412, 3413, 3414, 4096])
+def test_numbers_of_sequences(ph, dev, seqs):
+    """Around the number up to which a call's rows stand in shared memory."""
+    b = Both(ph, dev, n_pages=40, seqs=seqs, width=3, page=16, layers=1)
+    last = seqs - 1
+    assert b.extend([last], [20]) == 0
+    if seqs > 2:
+        assert b.fork([last], [0]) == 0 and b.extend([0, 1, last], [1, 40, 1]) == 0
+        assert b.fork([1], [2], deep=True) == 0
+    b.free([last])
+    b.compact()
+
+
 def test_refusals(ph, dev):
     import torch
     b = Both(ph, dev)
@@ -251,7 +264,10 @@ def test_refusals(ph, dev):
            lambda: ph.kv4_extend(b.cache, b.ints(list(range(13))), b.ints([0] * 13), b.out, workspace=b.ws),
            lambda: ph.kv4_fork(b.cache, one, one, b.out, workspace=torch.empty(1 << 20, dtype=torch.uint8, device=dev)[8:]),
            lambda: ph.kv4_compact(b.cache, torch.empty(0, dtype=torch.int32, device=dev), workspace=b.ws), lambda: ph.kv4_compact(b.cache, b.out),
-           lambda: ph.kv4_free(b.cache, b.ints([1, 2]), one)]
+           lambda: ph.kv4_free(b.cache, b.ints([1, 2]), one), lambda: ph.kv4_free(b.cache, None), lambda: ph.kv4_extend(b.cache, None, one, b.out, workspace=b.ws),
+           lambda: ph.kv4_extend(b.cache, one, None, b.out, workspace=b.ws), lambda: ph.kv4_extend(b.cache, one, one, None, workspace=b.ws),
+           lambda: ph.kv4_fork(b.cache, one, None, b.out, workspace=b.ws), lambda: ph.kv4_compact(b.cache, None, workspace=b.ws),
+           lambda: ph.kv4_extend(b.cache, one.cpu(), one, b.out, workspace=b.ws), lambda: ph.kv4_extend(b.cache, b.ints([1, 2, 3])[::2], b.ints([1, 1]), b.out, workspace=b.ws)]
     for f in bad:
         with pytest.raises(ph.PhobosError):
             f()
