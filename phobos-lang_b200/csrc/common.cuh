@@ -148,6 +148,16 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, u
   return mbar_wait_warp(bar, parity, site, ctx);
 }
 
+// mbar_wait_soon for a phase that copies into shared memory complete.  Where it gives up, the copies are waited for once
+// more, for a second and on a flag of its own, so that the CTA does not end while they may still be on their way.
+__device__ __forceinline__ bool mbar_wait_copies(uint64_t* bar, uint32_t parity, uint32_t site, const WaitCtx& ctx,
+                                                 volatile uint32_t* second_flag) {
+  if (mbar_wait_soon(bar, parity, site, ctx)) return true;
+  const WaitCtx again{second_flag, ctx.status, 1000000000ull};
+  mbar_wait_warp(bar, parity, site, again);
+  return false;
+}
+
 // Waits executed by a whole warp ahead of warp-collective TMEM accesses.
 #ifndef PH_WAIT_ALL_LANES
 #define PH_WARP_WAIT(bar, parity, site, ctx) mbar_wait_warp(bar, parity, site, ctx)

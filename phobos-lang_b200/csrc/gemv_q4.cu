@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(GV_THREADS, GV_PER_SM) gemv_q4_kernel(GemvPara
     mbar_init(full + threadIdx.x, 1);
     mbar_init(empty + threadIdx.x, GV_WARPS);
   }
-  if (threadIdx.x == 0) *abort_flag = 0;
+  if (threadIdx.x == 0) abort_flag[0] = abort_flag[1] = 0;
   fence_mbar_init();
   __syncthreads();
   pdl_wait();
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(GV_THREADS, GV_PER_SM) gemv_q4_kernel(GemvPara
 #pragma unroll 1
     for (int c = 0; c < chunks; c++) {
       const int kb = c * S::WK + wk;
-      const bool ok = mbar_wait_soon(full + st, parity, SITE_GEMV_FULL, ctx);  // else recorded; nothing hangs
+      const bool ok = mbar_wait_copies(full + st, parity, SITE_GEMV_FULL, ctx, abort_flag + 1);  // else recorded; nothing hangs
       const uint8_t* stage = ring + st * p.stage_bytes;
       auto block = [&](auto whole) {  // (behind K a stage holds whatever it held)
         const uint8_t* x_at = stage + x_row + wk * 256 + t * 16;

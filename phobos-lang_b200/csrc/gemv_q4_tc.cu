@@ -107,10 +107,10 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
   uint64_t* d_empty = d_full + QT_D_SLOTS;
   uint32_t* abort_flag = reinterpret_cast<uint32_t*>(d_empty + QT_D_SLOTS);
   uint32_t* tmem_slot = abort_flag + 1;
-  static_assert((3 * S::STAGES + 2 * QT_A_SLOTS + 2 * QT_D_SLOTS) * 8 + 8 <= S::HEAD, "barriers");
+  static_assert((3 * S::STAGES + 2 * QT_A_SLOTS + 2 * QT_D_SLOTS) * 8 + 16 <= S::HEAD, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
+    abort_flag[0] = abort_flag[2] = 0;  // (the word between them is tensor memory's address)
     for (int i = 0; i < S::STAGES; i++) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 8 + 4 + 2);       // widening, scaling (who have seen the products done) and summing warps
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
     Turn s;
     const int g = lane >> 2, t = lane & 3, block = warp - 14;
     for (int kb = kb0; kb < kb1; kb += QT_KBS, s.next(S::STAGES)) {
-      if (mbar_wait_soon(full + s.slot, s.parity, SITE_QT_FULL, ctx) && kb + block < kb1) {
+      if (mbar_wait_copies(full + s.slot, s.parity, SITE_QT_FULL, ctx, abort_flag + 2) && kb + block < kb1) {
         const uint8_t* x = ring + s.slot * S::STAGE + block * 2 * S::X_BOX;
         float* out = sums + (s.slot * QT_KBS + block) * S::GROUPS * NC;
 #pragma unroll
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
       a.slot = set;
       for (int kb = kb0; kb < kb1; kb += 2, s.next(S::STAGES)) {
         if (kb + set < kb1) {
-        const bool ok = mbar_wait_soon(full + s.slot, s.parity, SITE_QT_FULL, ctx);
+        const bool ok = mbar_wait_copies(full + s.slot, s.parity, SITE_QT_FULL, ctx, abort_flag + 2);
         const bool ok_a = kb < kb0 + QT_A_SLOTS || mbar_wait_soon(a_empty + a.slot, a.parity ^ 1, SITE_QT_A_EMPTY, ctx);
         if (ok && ok_a) {
           tc_fence_after_sync();
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
       Turn s, d;
       for (int kb = kb0; kb < kb1; kb++) {
         const int in_stage = (kb - kb0) % QT_KBS, groups = groups_of(kb);
-        bool ok = in_stage != 0 || (mbar_wait_soon(full + s.slot, s.parity, SITE_QT_FULL, ctx) &&
+        bool ok = in_stage != 0 || (mbar_wait_copies(full + s.slot, s.parity, SITE_QT_FULL, ctx, abort_flag + 2) &&
                                     mbar_wait_soon(summed + s.slot, s.parity, SITE_QT_SUMS, ctx));
         const __half2* par = reinterpret_cast<const __half2*>(ring + s.slot * S::STAGE + S::X_BYTES + tile * S::PITCH + in_stage * S::BLOCK + 1024) +
                              high * 8 + g;

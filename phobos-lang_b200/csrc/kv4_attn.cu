@@ -325,12 +325,12 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);                 // [AT_WARPS][STAGES]
   uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + 192);
-  static_assert(AT_WARPS * STAGES * 8 <= 192 && 196 <= S::HEAD, "shared memory head");
+  static_assert(AT_WARPS * STAGES * 8 <= 192 && 200 <= S::HEAD, "shared memory head");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + S::HEAD + warp * S::RING;
   uint64_t* bar = bars + warp * STAGES;
   if (threadIdx.x < AT_WARPS * STAGES) mbar_init(bars + threadIdx.x, 1);
-  if (threadIdx.x == 0) *abort_flag = 0;
+  if (threadIdx.x == 0) abort_flag[0] = abort_flag[1] = 0;
   fence_mbar_init();
   __syncthreads();
   pdl_wait();
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
 #pragma unroll 1
       for (int i = 0; i < n_tiles; i++) {
         const uint32_t n = phase + i, st = n % STAGES, here = (present >> (st * UN)) & ((1u << UN) - 1);
-        if (!mbar_wait_soon(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx)) continue;  // recorded; nothing hangs
+        if (!mbar_wait_copies(bar + st, (n / STAGES) & 1, SITE_KV4_RING, ctx, abort_flag + 1)) continue;  // recorded; nothing hangs
         const int tok0 = (w0 + i * UN) * KV4_UNIT;
         const uint8_t* stage = ring + st * S::STAGE;
         if (tok0 >= all_lo && tok0 + UN * KV4_UNIT <= all_hi && here == (1u << UN) - 1)
