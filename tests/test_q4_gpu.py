@@ -100,6 +100,42 @@ def test_alpha_beta_strides_and_columns_behind_n(ph, dev):
         assert bool(torch.isfinite(buf[:, 3:3 + N]).all()) and bool(torch.isnan(buf[:, :3]).all())
 
 
+def test_tensor_core_form_strides_alpha_beta_and_graph(ph, dev):
+    """The same where more than eight rows take the tensor-core form: rows of X out of a wider tensor, rows of Y too."""
+    import torch
+    M, N, K, G = 24, 16400, 4096, 128
+    code, scale, zero = _weights(N, K, G, 2, dev)
+    w = ph.q4_pack(code, scale, zero, G)
+    wide = torch.randn(M, K + 128, device=dev).half()
+    x = wide[:, 64:64 + K]
+    want, S = _want(x, code, scale, zero, G)
+    for dt in (torch.float16, torch.float32):
+        buf = torch.randn(M + 1, N + 9, device=dev).to(dt)
+        before = buf.clone()
+        ph.gemv_q4(x, w, buf[:M, 5:5 + N], G, alpha=-1.5, beta=0.5)
+        old = before[:M, 5:5 + N].double()
+        tol = _tol(1.5 * S + 0.5 * old.abs(), -1.5 * want + 0.5 * old, K, G, dt == torch.float16)
+        assert bool(((buf[:M, 5:5 + N].double() - (-1.5 * want + 0.5 * old)).abs() <= tol).all())
+        assert torch.equal(buf[M:], before[M:]) and torch.equal(buf[:, :5], before[:, :5]) and torch.equal(buf[:, 5 + N:], before[:, 5 + N:])
+    y, z = torch.empty(M, N, device=dev), torch.empty(M, N, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    ph.gemv_q4(x, w, z, G)
+    with torch.cuda.graph(graph):
+        ph.gemv_q4(x, w, z, G)
+        ph.gemv_q4(x[:7], w, z[:7], G)       # the other form right behind it
+    wide.mul_(-0.5)
+    graph.replay()
+    ph.gemv_q4(x, w, y, G)
+    ph.gemv_q4(x[:7], w, y[:7], G)
+    assert torch.equal(y, z)
+    # an infinity in one row of X stays there
+    x[3, 9] = float("inf")
+    ph.gemv_q4(x, w, y, G)
+    keep = [i for i in range(M) if i != 3]
+    assert torch.equal(y[keep][7:], z[keep][7:]) and bool(torch.isfinite(y[keep]).all()) and not bool(torch.isfinite(y[3]).any())
+    assert ph.device_status() == 0
+
+
 def test_extreme_values(ph, dev):
     """f16's largest and smallest x and scales: no product leaves f32, subnormals are not flushed."""
     import torch
