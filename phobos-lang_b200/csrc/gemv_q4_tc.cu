@@ -249,30 +249,32 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
       const int set = warp >> 2;
       a.slot = set;
       for (int kb = kb0; kb < kb1; kb += 2, s.next(S::STAGES)) {
-        if (kb + set < kb1) {
+        // Both sets wait for every stage, the last one with a single block too: an arrival on `empty` for a stage that has not
+        // come would count for the one before it in the slot, whose (scale, zero) pairs and sums are still being read.
         const bool ok = mbar_wait_copies(full + s.slot, s.parity, SITE_QT_FULL, ctx, abort_flag + 2);
-        const bool ok_a = kb < kb0 + QT_A_SLOTS || mbar_wait_soon(a_empty + a.slot, a.parity ^ 1, SITE_QT_A_EMPTY, ctx);
-        if (ok && ok_a) {
-          tc_fence_after_sync();
-          const uint8_t* row = ring + s.slot * S::STAGE + S::X_BYTES + tile * S::PITCH + set * S::BLOCK + g * 64;
+        if (kb + set < kb1) {
+          const bool ok_a = kb < kb0 + QT_A_SLOTS || mbar_wait_soon(a_empty + a.slot, a.parity ^ 1, SITE_QT_A_EMPTY, ctx);
+          if (ok && ok_a) {
+            tc_fence_after_sync();
+            const uint8_t* row = ring + s.slot * S::STAGE + S::X_BYTES + tile * S::PITCH + set * S::BLOCK + g * 64;
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            uint32_t c[32];  // 64 columns of W
+            for (int half = 0; half < 2; half++) {
+              uint32_t c[32];  // 64 columns of W
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-              const uint4 v = *reinterpret_cast<const uint4*>(row + half * 512 + t * 16);
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              for (int t = 0; t < 4; t++) {
+                const uint4 v = *reinterpret_cast<const uint4*>(row + half * 512 + t * 16);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int j = 0; j < 4; j++) {
-                c[16 * (j >> 1) + 4 * t + 2 * (j & 1)] = w[j] & mask;
-                c[16 * (j >> 1) + 4 * t + 2 * (j & 1) + 1] = (w[j] >> 8) & mask;
+                for (int j = 0; j < 4; j++) {
+                  c[16 * (j >> 1) + 4 * t + 2 * (j & 1)] = w[j] & mask;
+                  c[16 * (j >> 1) + 4 * t + 2 * (j & 1) + 1] = (w[j] >> 8) & mask;
+                }
               }
+              tmem_st_32x32b_x32(tmem_a + a.slot * QT_A_COLS + half * 32 + tmem_row, c);
             }
-            tmem_st_32x32b_x32(tmem_a + a.slot * QT_A_COLS + half * 32 + tmem_row, c);
+            tmem_st_wait();
+            tc_fence_before_sync();
           }
-          tmem_st_wait();
-          tc_fence_before_sync();
-        }
           __syncwarp();
           if (lane == 0) mbar_arrive(a_full + a.slot);
           a.next(QT_A_SLOTS);

@@ -201,3 +201,22 @@ def test_refusals(ph, dev):
             f()
     ph.gemv_q4(x[:0], w, y[:0], G)   # no rows: nothing to do
     assert ph.device_status() == 0
+
+
+@pytest.mark.parametrize("M,N,K,G", [(64, 16384, 1152, 128), (64, 4096, 5504, 128), (64, 4096, 13696, 128)])
+def test_tensor_core_form_with_a_half_filled_last_stage(ph, dev, M, N, K, G):
+    """An odd number of 128-column blocks, or an odd share of them for each CTA of a cluster of two: the last stage holds one
+    block instead of two, which must not release the stage before it in its slot.  The same bits in every call."""
+    import torch
+    g = torch.Generator().manual_seed(K)
+    x = torch.randn(M, K, generator=g).half().to(dev)
+    code, scale, zero = _weights(N, K, G, N + K, dev)
+    w = ph.q4_pack(code, scale, zero, G)
+    y, again = torch.empty(M, N, device=dev), torch.empty(M, N, device=dev)
+    ph.gemv_q4(x, w, y, G)
+    want, S = _want(x, code, scale, zero, G)
+    assert bool(((y.double() - want).abs() <= _tol(S, want, K, G, False)).all())
+    for _ in range(30):
+        ph.gemv_q4(x, w, again, G)
+        assert torch.equal(y, again)
+    assert ph.device_status() == 0
