@@ -228,6 +228,9 @@ int phobos_kv4_attention(const PhKv4Cache* cache, int32_t layer, const PhTensor*
   if (lse && (l.rows != q.rows || l.cols != q_heads))
     return fail(PH_ERR_INVALID, "kv4_attention: lse %lldx%lld, expected %lldx%lld", l.rows, l.cols, q.rows, q_heads);
   if (window < 0) return fail(PH_ERR_INVALID, "kv4_attention: window %d", window);
+  // No sequence is longer than its table, so a window of that size hides nothing.  (The kernel takes windows from positions,
+  // which are negative for rows in front of a sequence's first token: below 2^28 the difference stays within 32 bits.)
+  if (window >= static_cast<long long>(c.table_width) << c.page_shift) window = 0;
   if ((rc = batch_of("kv4_attention", slots, indptr, n, q.rows))) return rc;
   const long long T = indptr ? q.rows : n;
   const size_t need = kv4_attention_workspace(c, static_cast<int>(T), n, static_cast<int>(q_heads), sm_count_or_default());

@@ -480,3 +480,12 @@ def test_refusals(ph, dev):
             print("not refused:", i)
     att()
     assert ph.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 7, 10 ** 6, 97, 96, 95])
+def test_windows_that_hide_nothing_or_little(ph, dev, window):
+    """The largest windows, with more rows than tokens among the sequences, and windows around what the tables hold (96)."""
+    s = Setup(ph, dev, [5, 70, 1, 80], 2, 64, 64, 16, seed=11)
+    assert s.cache.tables.shape[1] * 16 == 96
+    check(s, [9, 70, 4, 1], 4, window=window)
+    check(s, [1, 1, 1, 1], 4, window=window, seed=2)
