@@ -259,10 +259,10 @@ PH_API int phobos_kv4_read(const PhKv4Cache *cache, int32_t layer, const PhTenso
 
 /* O = softmax(scale * q K^T) V over the cache.  Q, O: [T, q_heads * head_dim] f16, q_heads a multiple of kv_heads
  * (head h reads key/value head h / (q_heads / kv_heads)).  The row of position p sees tokens j <= p, and with
- * window > 0 only j > p - window.  A row that sees nothing gets zeros.  lse, [T, q_heads] f32 or NULL: the natural
- * logarithm of the sum of exp(scale * q k), -inf for a row that sees nothing.  The workspace (256-byte aligned,
- * phobos_kv4_attention_workspace_bytes; its contents need not be kept) holds what is found of one sequence in several places;
- * calls that share one must not overlap on the GPU. */
+ * window > 0 only j > p - window.  A row that sees nothing gets zeros.  O is at most +-65504, as values read back are.
+ * lse, [T, q_heads] f32 or NULL: the natural logarithm of the sum of exp(scale * q k), -inf for a row that sees nothing.
+ * The workspace (256-byte aligned, phobos_kv4_attention_workspace_bytes; its contents need not be kept) holds what is
+ * found of one sequence in several places; calls that share one must not overlap on the GPU. */
 PH_API size_t phobos_kv4_attention_workspace_bytes(const PhKv4Cache *cache, int64_t T, int32_t n, int32_t q_heads);
 PH_API int phobos_kv4_attention(const PhKv4Cache *cache, int32_t layer, const PhTensor *Q, const PhTensor *O,
                                 const PhTensor *lse, float scale, int32_t window, const int32_t *slots,

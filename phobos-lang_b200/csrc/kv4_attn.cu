@@ -46,6 +46,14 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2^n for -126 <= n <= 127
 __device__ __forceinline__ float pow2i(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
 
+// Rounded to f16, at most +-65504 in size as kv4_read has it: zero + 15 step can pass the group's largest value by the
+// rounding of the step, and must not become an infinity (a NaN stays).
+__device__ __forceinline__ uint32_t pack_output(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* at) {
   if constexpr (N == 4) {
@@ -534,7 +542,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 3 : D == 64 ? 3 : 2) 
           }
           if (whole)
             *reinterpret_cast<uint2*>(static_cast<__half*>(p.a.O) + out * p.a.ldo + h * D + 32 * i + 4 * g) =
-                make_uint2(pack_half2(v[0] * inv, v[1] * inv), pack_half2(v[2] * inv, v[3] * inv));
+                make_uint2(pack_output(v[0] * inv, v[1] * inv), pack_output(v[2] * inv, v[3] * inv));
           else
             *reinterpret_cast<float4*>(part + in_tile * D + 32 * i + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
         }
@@ -634,7 +642,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, in
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     __half* to = static_cast<__half*>(p.a.O) + out * p.a.ldo + h * D + lane * DIMS;
 #pragma unroll
-    for (int d = 0; d < DIMS; d += 2) *reinterpret_cast<__half2*>(to + d) = __floats2half2_rn(o[d] * inv, o[d + 1] * inv);
+    for (int d = 0; d < DIMS; d += 2) *reinterpret_cast<uint32_t*>(to + d) = pack_output(o[d] * inv, o[d + 1] * inv);
     if (lane == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
   }
   if (!__syncthreads_or(longer)) return;
@@ -679,7 +687,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(AttnParams p, in
       long long out;
       int h;
       place(cut, r, &out, &h);
-      static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __float2half_rn(l == 0.0f ? 0.0f : o / l);
+      static_cast<__half*>(p.a.O)[out * p.a.ldo + h * D + d] = __ushort_as_half(static_cast<uint16_t>(pack_output(l == 0.0f ? 0.0f : o / l, 0.0f)));
       if (d == 0 && p.a.lse) p.a.lse[out * p.a.ldl + h] = l == 0.0f ? -INFINITY : fmaf(m, LN2, logf(l));
     }
     __syncthreads();

@@ -489,3 +489,28 @@ def test_windows_that_hide_nothing_or_little(ph, dev, window):
     assert s.cache.tables.shape[1] * 16 == 96
     check(s, [9, 70, 4, 1], 4, window=window)
     check(s, [1, 1, 1, 1], 4, window=window, seed=2)
+
+
+@pytest.mark.parametrize("length", [1, 700, 20000])
+def test_values_over_the_whole_range_give_finite_outputs(ph, dev, length):
+    """A group from -65504 to 65504 has the scale 8736 (131008 / 15 to f16), so that its code 15 stands for 65536: O has
+    65504 there, as kv4_read gives.  One token, parts joined by a warp a row, and parts joined by a block.
+    Weights off by 2^-11 of 8 scales either way leave code 15 above 65506 and code 0 within 8 * 8736 * 2^-11 < 35 and half an f16
+    step, 16, of -65504."""
+    import torch
+    D, G = 64, 32
+    s = Setup(ph, dev, [length], 1, D, G, 64, seed=12)
+    s.v[:, 0::2], s.v[:, 1::2] = 65504.0, -65504.0
+    ind = torch.tensor([0, length], dtype=torch.int32, device=dev)
+    ph.kv4_append(s.cache, 0, s.k, s.v, s.slots, ind)
+    k, v = torch.empty_like(s.k), torch.empty_like(s.v)
+    ph.kv4_read(s.cache, 0, k, v, s.slots, ind)
+    assert torch.equal(v, s.v)
+    o, lse = attend(s, torch.randn(1, 2 * D, device=dev).half(), [0, 1], 0.125)
+    assert ph.device_status() == 0 and bool(torch.isfinite(lse).all())
+    assert bool((o[:, 0::2] == 65504.0).all()) and bool(((o[:, 1::2].float() + 65504.0).abs() <= 35 + 16).all())
+    # a NaN is none of those
+    s.v[0, 3] = float("nan")
+    ph.kv4_append(s.cache, 0, s.k, s.v, s.slots, ind)
+    o, _ = attend(s, torch.randn(1, 2 * D, device=dev).half(), [0, 1], 0.125)
+    assert bool(torch.isnan(o.view(2, D)[:, :G]).all()) and bool(torch.isfinite(o.view(2, D)[:, G:]).all())
