@@ -201,6 +201,7 @@ PH_API int phobos_saxpy(const PhTensor *x, const PhTensor *y, const PhTensor *ou
  * Y[M,N] = alpha * X[M,K] W[N,K]^T + beta * Y with W[n,k] = scale[n,k/group] *
  * (code[n,k] - zero[n,k/group]), codes 0..15, group 32, 64 or 128, K a multiple of group.
  * X is f16, Y f16 or f32 (f32 sums, rounded once); Y is not read when beta == 0.
+ * An infinity in X makes of its row of Y what the formula says: an infinity, or NaN where it meets a weight of zero.
  * X: rows 16-byte aligned.  Y: any N, any row stride >= N.
  * phobos_q4_pack lays weights out once, in the order the kernel reads them: codes [N,K] one
  * per byte (the low four bits count), scales and zeros [N, K/group] f16 (zeros may be NULL:

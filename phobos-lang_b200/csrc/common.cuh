@@ -415,5 +415,20 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// The same, and whether any of those threads brings `value`.
+__device__ __forceinline__ bool named_bar_or(int id, int threads, bool value) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      "setp.ne.u32 P, %3, 0;\n\t"
+      "barrier.cta.red.or.pred Q, %1, %2, P;\n\t"
+      "selp.u32 %0, 1, 0, Q;\n\t"
+      "}\n"
+      : "=r"(any)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(value))
+      : "memory");
+  return any != 0;
+}
 
 }  // namespace ph

@@ -2,7 +2,8 @@
 //
 //   sum_k x_k s (c_k - z) = s ( sum_k x_k c_k - z sum_k x_k )      within a group of G columns
 // so the matrix unit sees the bare codes, a group's sum is scaled once in f32, and nothing is rounded between X and Y
-// but the f32 sums.
+// but the f32 sums.  Where infinities in X make the two sums cancel to NaN, the sum is formed from the definition
+// (q4_not_finite).
 //
 // Packed weights: blocks of 16 rows x 128 columns, [N / 16][K / 128], each 1024 bytes of codes and then [128 / G][16]
 // (scale, zero) pairs of f16.  Lane 4g + t of a warp finds in words w = 2 S + e (bytes (w / 4) * 512 + lane * 16 +
@@ -195,24 +196,37 @@ __global__ void __launch_bounds__(GV_THREADS, GV_PER_SM) gemv_q4_kernel(GemvPara
     for (int r = 0; r < RT; r++)
 #pragma unroll
       for (int i = 0; i < 4; i++) out[(wk * 8 + 2 * t + (i & 1)) * S::OUT_PITCH + (r * WR + wr) * 16 + g + (i >> 1) * 8] = y[r][i];
-    named_bar_sync(1, GV_WARPS * 32);
-    const int n_rows = min(min(S::TILES, last - tile0) * 16, p.N - tile0 * 16);
-    for (int i = threadIdx.x; i < n_m * S::ROWS; i += GV_WARPS * 32) {
-      const int row = i % S::ROWS, col = i / S::ROWS;
-      if (row >= n_rows) continue;
-      float v = 0.0f;
+    bool nan = false;
 #pragma unroll
-      for (int k = 0; k < S::WK; k++) v += out[(k * 8 + col) * S::OUT_PITCH + row];
-      v *= p.alpha;
-      const long long at = (m0 + col) * p.ldy + tile0 * 16 + row;
-      if (p.out_f32) {
-        float* o = static_cast<float*>(p.Y) + at;
-        *o = p.beta == 0.0f ? v : fmaf(p.beta, *o, v);
-      } else {
-        __half* o = static_cast<__half*>(p.Y) + at;
-        *o = __float2half_rn(p.beta == 0.0f ? v : fmaf(p.beta, __half2float(*o), v));
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) nan = nan || y[r][i] != y[r][i];
+    nan = named_bar_or(1, GV_WARPS * 32, nan);
+    const int n_rows = min(min(S::TILES, last - tile0) * 16, p.N - tile0 * 16);
+    auto write = [&](auto look) {
+      for (int i = threadIdx.x; i < n_m * S::ROWS; i += GV_WARPS * 32) {
+        const int row = i % S::ROWS, col = i / S::ROWS;
+        if (row >= n_rows) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < S::WK; k++) v += out[(k * 8 + col) * S::OUT_PITCH + row];
+        if (decltype(look)::value && v != v)
+          v = q4_not_finite(v, p.X + (m0 + col) * p.ldx, p.W, tile0 * 16 + row, p.K, p.kblocks, GS * 16);
+        v *= p.alpha;
+        const long long at = (m0 + col) * p.ldy + tile0 * 16 + row;
+        if (p.out_f32) {
+          float* o = static_cast<float*>(p.Y) + at;
+          *o = p.beta == 0.0f ? v : fmaf(p.beta, *o, v);
+        } else {
+          __half* o = static_cast<__half*>(p.Y) + at;
+          *o = __float2half_rn(p.beta == 0.0f ? v : fmaf(p.beta, __half2float(*o), v));
+        }
       }
-    }
+    };
+    if (__builtin_expect(nan, 0))
+      write(std::true_type{});
+    else
+      write(std::false_type{});
     named_bar_sync(1, GV_WARPS * 32);
   }
 }

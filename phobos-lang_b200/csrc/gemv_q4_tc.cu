@@ -36,9 +36,10 @@ enum : uint32_t {
 };
 
 struct TcGemvParams {
+  const __half* X;
   const uint8_t* W;
   void* Y;
-  long long ldy;
+  long long ldx, ldy;
   int M, N, K, kblocks, tiles, tiles_per_cta, split;       // split: CTAs of a cluster, along K
   float alpha, beta;
   int out_f32;
@@ -346,11 +347,26 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
     }
   };
   const int n_m = min(NC, p.M - m0);
+  auto not_finite = [&](int m, float v) { return q4_not_finite(v, p.X + (m0 + m) * p.ldx, p.W, n, p.K, p.kblocks, GS * 16); };
   if (p.split == 1) {
-    if (mine)
+    if (mine) {
+      bool nan = false;
 #pragma unroll
-      for (int m = 0; m < NC; m++)
-        if (m < n_m) write(m, y[m]);
+      for (int m = 0; m < NC; m++) nan = nan || y[m] != y[m];
+      if (!nan) {
+#pragma unroll
+        for (int m = 0; m < NC; m++)
+          if (m < n_m) write(m, y[m]);
+      } else {
+#pragma unroll 1
+        for (int m = 0; m < n_m; m++) {
+          float v = 0.0f;
+#pragma unroll
+          for (int i = 0; i < NC; i++) v = i == m ? y[i] : v;  // (y stays in registers)
+          write(m, v == v ? v : not_finite(m, v));
+        }
+      }
+    }
   } else {
     constexpr int PITCH = NC + 4;
     float* red = reinterpret_cast<float*>(ring);
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) gemv_q4_tc_kernel(const __grid_
       for (int m = rank; m < n_m; m += p.split) {  // this CTA's columns
         float v = 0.0f;
         for (int r = 0; r < p.split; r++) v += ld_cluster_f32(mapa_u32(at + m * 4, r));
-        write(m, v);
+        write(m, v == v ? v : not_finite(m, v));
       }
     }
     __syncwarp();
@@ -472,7 +488,7 @@ int launch_gemv_q4_tc(const void* X, long long ldx, const void* W, void* Y, long
     *err = "gemv_q4: too many rows of X";
     return -2;
   }
-  TcGemvParams p{static_cast<const uint8_t*>(W), Y, ldy, M, N, K, (K + 127) / 128, (N + 15) / 16, 0, 0, alpha, beta, out_f32, status};
+  TcGemvParams p{static_cast<const __half*>(X), static_cast<const uint8_t*>(W), Y, ldx, ldy, M, N, K, (K + 127) / 128, (N + 15) / 16, 0, 0, alpha, beta, out_f32, status};
   return group == 128  ? launch_group<8>(X, ldx, p, sm_count, stream, err)
          : group == 64 ? launch_group<4>(X, ldx, p, sm_count, stream, err)
                        : launch_group<2>(X, ldx, p, sm_count, stream, err);

@@ -220,3 +220,37 @@ def test_tensor_core_form_with_a_half_filled_last_stage(ph, dev, M, N, K, G):
         ph.gemv_q4(x, w, again, G)
         assert torch.equal(y, again)
     assert ph.device_status() == 0
+
+
+@pytest.mark.parametrize("M,N,K,G", [(5, 70, 256, 32), (8, 5000, 384, 128), (1, 24, 16384, 64), (24, 16400, 1024, 128), (11, 16387, 512, 64), (64, 4100, 5504, 128),
+                                     (64, 2048, 8192, 128)])
+@pytest.mark.parametrize("out", ["f16", "f32"])
+def test_infinities_are_those_of_the_definition(ph, dev, M, N, K, G, out):
+    """inf and -inf in x, alone, in one group, in two, and a NaN: infinities of the weight's sign, NaN where a weight is zero or
+    infinities cancel, and the rows without any as they are."""
+    import torch
+    g = torch.Generator().manual_seed(N)
+    x = torch.randn(M, K, generator=g).half().to(dev)
+    code, scale, _ = _weights(N, K, G, N + K, dev)
+    zero = torch.randint(-3, 16, (N, K // G), generator=g).half().to(dev)
+    scale[::3] *= -1
+    scale[5] = 0
+    inf = float("inf")
+    x[0, 17] = inf
+    if M > 4:
+        x[1, K - 1] = -inf
+        x[2, 3], x[2, 9], x[2, K - 20] = inf, -inf, inf
+        x[3, 40], x[3, 41] = float("nan"), inf
+    y = torch.randn(M, N, device=dev).to(torch.float16 if out == "f16" else torch.float32)
+    old = y.double()
+    ph.gemv_q4(x, ph.q4_pack(code, scale, zero, G), y, G, alpha=-0.5, beta=0.25)
+    assert ph.device_status() == 0
+    want, _ = _want(x, code, scale, zero, G)
+    want = -0.5 * want + 0.25 * old
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    assert torch.equal(torch.isinf(y), torch.isinf(want)) and bool((y.double() == want)[torch.isinf(want)].all())
+    assert bool(torch.isinf(want[0]).any()) and bool(torch.isnan(want[0]).any())
+    ok = torch.isfinite(want)
+    _, S = _want(x, code, scale.abs(), zero, G)
+    S = 0.5 * S + 0.25 * old.abs()
+    assert bool(((y.double() - want).abs() <= _tol(S, want, K, G, out == "f16"))[ok].all())
