@@ -435,20 +435,8 @@ cudaError_t launch_shape(const CUtensorMap& x_map, TcGemvParams& p, int sm_count
   const TcGemvSplit s = tc_gemv_split(p.tiles, p.kblocks, m_groups, sm_count);
   p.tiles_per_cta = s.tiles_per_cta;
   p.split = s.split;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.tiles + p.tiles_per_cta - 1) / p.tiles_per_cta * p.split, m_groups);
-  cfg.blockDim = dim3(QT_THREADS);
-  cfg.dynamicSmemBytes = S::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, x_map, p);
+  return launch_clusters_with_pdl(kernel, dim3((p.tiles + p.tiles_per_cta - 1) / p.tiles_per_cta * p.split, m_groups), dim3(QT_THREADS), p.split,
+                                  S::SMEM, stream, x_map, p);
 }
 
 template <int GS>

@@ -9,8 +9,10 @@ namespace ph {
 // Launches `kernel` so that its prologue may overlap the tail of the kernel before it on the stream
 // (programmatic stream serialization); the kernel calls pdl_wait() before its first dependent access.
 // PHOBOS_PDL=0 falls back to an ordinary launch.
+// launch_clusters_with_pdl: the same in clusters of `cluster` CTAs along x.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_with_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+cudaError_t launch_clusters_with_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, unsigned cluster, size_t smem, cudaStream_t stream,
+                                     Args... args) {
   static const bool off = [] {
     const char* e = getenv("PHOBOS_PDL");
     return e && e[0] == '0';
@@ -20,12 +22,25 @@ cudaError_t launch_with_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (!off) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 0) {  // (0: the kernel is not one for clusters, or says itself of how many CTAs)
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    n++;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = off ? 0 : 1;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_with_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  return launch_clusters_with_pdl(kernel, grid, block, 0, smem, stream, args...);
 }
 
 

@@ -254,3 +254,45 @@ def test_infinities_are_those_of_the_definition(ph, dev, M, N, K, G, out):
     _, S = _want(x, code, scale.abs(), zero, G)
     S = 0.5 * S + 0.25 * old.abs()
     assert bool(((y.double() - want).abs() <= _tol(S, want, K, G, out == "f16"))[ok].all())
+
+
+EDGES = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+import __graft_entry__ as entry
+from cuda.bindings import runtime
+ph = entry.load_package()
+dev = torch.device("cuda:0")
+calls = []
+for M, N, K in ((24, 16400, 1024), (64, 2048, 8192), (3, 80, 512)):      # tcgen05, in clusters, warp-level
+    code = torch.randint(0, 16, (N, K), device=dev, dtype=torch.uint8)
+    w = ph.q4_pack(code, torch.rand(N, K // 128, device=dev).half(), None, 128)
+    calls.append((torch.randn(M, K, device=dev).half(), w, torch.empty(M, N, device=dev)))
+for c in calls:
+    ph.gemv_q4(*c, 128)
+graph = torch.cuda.CUDAGraph(keep_graph=True)
+with torch.cuda.graph(graph):
+    for c in calls + calls:
+        ph.gemv_q4(*c, 128)
+get = lambda *n: runtime.cudaGraphGetEdges_v2(runtime.cudaGraph_t(graph.raw_cuda_graph()), *n)
+n = get()[-1]
+_, _, _, data, _ = get(n)
+print("edges", n, sum(int(d.type) == int(runtime.cudaGraphDependencyType.cudaGraphDependencyTypeProgrammatic) for d in data))
+"""
+
+
+@pytest.mark.parametrize("pdl", ["0", "1"])
+def test_the_switch_for_early_starts_reaches_every_form(ph, dev, pdl):
+    """PHOBOS_PDL=0 (read once, so in a process of its own) turns the early start off for all of gemv_q4's kernels: of the
+    five edges between six captured calls none is then programmatic.  Without it some are (not all: capture puts ordinary
+    edges in front of kernels in clusters)."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = EDGES.replace("{root!r}", repr(str(Path(__file__).resolve().parent.parent)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=dict(os.environ, PHOBOS_PDL=pdl))
+    assert r.returncode == 0, r.stderr[-2000:]
+    word, edges, early = r.stdout.split()
+    assert (word, edges) == ("edges", "5") and (int(early) > 0) == (pdl == "1")
