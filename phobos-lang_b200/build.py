@@ -16,7 +16,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 LIB = HERE / "libphobos_leaf.so"
-BIND = HERE / "_bind.so"            # CPython module of serve.py's short calls
+# CPython module of serve.py's short calls; the suffix names the interpreter it was built for
+BIND = HERE / ("_bind" + sysconfig.get_config_var("EXT_SUFFIX") or ".so")
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_f32.cu", "flash.cu", "elementwise.cu", "kda.cu", "tmap.cu", "noalloc.cu", "selftest.cu",
            "gemv_q4.cu", "gemv_q4_tc.cu", "kv4_cache.cu", "kv4_attn.cu", "kv4_pages.cu", "serve_api.cu",
            "host.cpp", "executor.cpp", "source.cpp", "planner.cpp", "plan_api.cpp", "wire.cpp"]
@@ -40,14 +41,40 @@ def _deps_mtime() -> float:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     sources = [s for s in SOURCES if (CSRC / s).exists()]
-    if not force and all(so.exists() and so.stat().st_mtime >= _deps_mtime() for so in (LIB, BIND)):
-        return LIB
-    OBJ.mkdir(exist_ok=True)
-    nvcc = _nvcc()
+    newest = _deps_mtime()
+    current = lambda so: not force and so.exists() and so.stat().st_mtime >= newest  # noqa: E731
+    if not current(LIB):
+        _build_lib(sources, verbose)
+    if not current(BIND):
+        build_bind()
+    return LIB
+
+
+def _env() -> dict:
     env = dict(os.environ)
     # the environment may export CC/CXX pointing at a wrapper; nvcc should use the system g++
     env.pop("CC", None)
     env.pop("CXX", None)
+    return env
+
+
+def build_bind(out: Path = BIND, headers: str | None = None) -> Path | None:
+    """Builds serve.py's CPython module.  It is not part of the C library, which needs no Python: where this interpreter's
+    headers are not installed, that is said and None returned, and the calls that use the module raise ImportError."""
+    headers = headers or sysconfig.get_paths()["include"]
+    if not (Path(headers) / "Python.h").exists():
+        print(f"{out.name} not built: no Python.h in {headers} (the 4-bit calls of serve.py need it)", file=sys.stderr)
+        return None
+    r = subprocess.run([_nvcc(), "-O2", "-std=c++17", "-cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-shared", "-I", headers,
+                        str(CSRC / "bind.cpp"), "-o", str(out)], capture_output=True, text=True, env=_env())
+    if r.returncode != 0:
+        raise RuntimeError(f"nvcc failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
+    return out
+
+
+def _build_lib(sources: list[str], verbose: bool) -> None:
+    OBJ.mkdir(exist_ok=True)
+    nvcc, env = _nvcc(), _env()
 
     def compile_one(src: str) -> tuple[str, str]:
         obj = OBJ / (src.rsplit(".", 1)[0] + ".o")
@@ -69,11 +96,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     r = subprocess.run(link, capture_output=True, text=True, env=env)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    r = subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
-                        str(CSRC / "bind.cpp"), "-o", str(BIND)], capture_output=True, text=True, env=env)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
-    return LIB
 
 
 if __name__ == "__main__":

@@ -161,3 +161,27 @@ def test_launch_by_name_needs_the_group(ph):
     g = (ctypes.c_uint32 * 3)(1, 1, 1)
     refused(ph, ph.lib().phobos_launch(b"gemv_q4", t, 3, s, 2, g, g, -1, None, 0, None), ph.PH_ERR_INVALID)
     refused(ph, ph.lib().phobos_launch(b"gemv_q4", t, 2, s, 2, g, g, -1, None, 0, None), ph.PH_ERR_INVALID)
+
+
+def test_the_short_calls_module_names_its_interpreter_and_is_left_out_without_headers(ph, tmp_path, capfd, monkeypatch):
+    """The C library's build asks for no Python; the CPython module carries the interpreter's suffix, so that another
+    interpreter does not load it, and without headers the library is all that is built."""
+    import sysconfig
+
+    import __graft_entry__ as entry
+    build = entry._load_build_module()
+    assert build.BIND.name == "_bind" + sysconfig.get_config_var("EXT_SUFFIX") != "_bind.so"
+    assert build.build_bind(tmp_path / "x.so", headers=str(tmp_path)) is None
+    assert "Python.h" in capfd.readouterr().err and not list(tmp_path.iterdir())
+    # a build asks for the module apart from the library, and ends well without it
+    monkeypatch.setattr(build, "BIND", tmp_path / "y.so")
+    calls = []
+    monkeypatch.setattr(build, "_build_lib", lambda *a: None)
+    monkeypatch.setattr(build, "build_bind", lambda: calls.append(1))
+    assert build.build() == build.LIB and calls == [1]
+    # the calls then say what is missing
+    from phobos_lang_b200 import serve
+    monkeypatch.setattr(serve, "_bind", None)
+    monkeypatch.setattr(serve, "LIB_PATH", tmp_path / "libphobos_leaf.so")
+    with pytest.raises(ImportError, match="_bind"):
+        serve.gemv_q4(None, None, None, 64)
