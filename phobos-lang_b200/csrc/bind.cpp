@@ -4,6 +4,7 @@
 // serve.py hands it the entry points' addresses, torch's types and the exception to raise.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <pthread.h>
 
 #include <cstdint>
 
@@ -158,6 +159,21 @@ bool cache_of(PyObject* pair, const Call& c, const PhKv4Cache** cache) {
   return !PyErr_Occurred() && refuse(PH_ERR_INVALID, "%s does not live on the current device", "the cache");
 }
 
+// Calls an entry point without the interpreter's lock: a launch waits where the stream's queue is full, and what it waits for
+// may be a host function of the stream that needs the lock.  A lock of its own keeps the launches of one call together, so
+// that threads which share a stream and a workspace still make their calls one after another.
+pthread_mutex_t g_calls = PTHREAD_MUTEX_INITIALIZER;
+
+template <typename F>
+PyObject* unlocked(F call) {
+  PyThreadState* state = PyEval_SaveThread();
+  pthread_mutex_lock(&g_calls);
+  const int rc = call();
+  pthread_mutex_unlock(&g_calls);
+  PyEval_RestoreThread(state);
+  return PyLong_FromLong(rc);
+}
+
 bool args_are(Py_ssize_t n, Py_ssize_t want) {
   if (n == want) return true;
   PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
@@ -173,7 +189,9 @@ PyObject* gemv_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!args_are(n, 7) || !begin(a[6], &c) || !describe(a[0], "X", c, &x) || !describe(a[1], "packed", c, &w) || !describe(a[2], "Y", c, &y) ||
       !whole(a[3], &group) || !real(a[4], &alpha) || !real(a[5], &beta))
     return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_gemv_q4)>(g_entry[GEMV_Q4])(&x, &w, &y, alpha, beta, group, c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_gemv_q4)>(g_entry[GEMV_Q4])(&x, &w, &y, alpha, beta, group, c.stream);
+  });
 }
 
 // rows(read, cache, layer, K, V, slots, indptr, stream)
@@ -186,8 +204,10 @@ PyObject* rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!args_are(n, 8) || !begin(a[7], &c) || !whole(a[0], &read) || !cache_of(a[1], c, &cache) || !whole(a[2], &layer) || !describe(a[3], "K", c, &k) ||
       !describe(a[4], "V", c, &v) || !integers(a[5], "slots", c, 0, &slots, &count) || !integers(a[6], "indptr", c, count + 1, &indptr))
     return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_kv4_append)>(g_entry[read ? KV4_READ : KV4_APPEND])(
-      cache, layer, &k, &v, slots, indptr, static_cast<int32_t>(count), c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_kv4_append)>(g_entry[read ? KV4_READ : KV4_APPEND])(
+        cache, layer, &k, &v, slots, indptr, static_cast<int32_t>(count), c.stream);
+  });
 }
 
 // attention(cache, layer, Q, O, lse, scale, window, slots, indptr, workspace, stream)
@@ -204,8 +224,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !describe(a[3], "O", c, &o) || (a[4] != Py_None && !describe(a[4], "lse", c, &lse)) || !real(a[5], &scale) || !whole(a[6], &window) ||
       !integers(a[7], "slots", c, 0, &slots, &count) || !integers(a[8], "indptr", c, count + 1, &indptr) || !space(a[9], c, &ws, &bytes))
     return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_kv4_attention)>(g_entry[KV4_ATTENTION])(
-      cache, layer, &q, &o, a[4] != Py_None ? &lse : nullptr, scale, window, slots, indptr, static_cast<int32_t>(count), ws, bytes, c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_kv4_attention)>(g_entry[KV4_ATTENTION])(
+        cache, layer, &q, &o, a[4] != Py_None ? &lse : nullptr, scale, window, slots, indptr, static_cast<int32_t>(count), ws, bytes, c.stream);
+  });
 }
 
 // extend(cache, slots, counts, shortfall, workspace, stream)
@@ -219,8 +241,10 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!args_are(n, 6) || !begin(a[5], &c) || !cache_of(a[0], c, &cache) || !integers(a[1], "slots", c, 0, &slots, &count) ||
       !integers(a[2], "counts", c, count, &counts) || !integers(a[3], "shortfall", c, 1, &shortfall) || !space(a[4], c, &ws, &bytes))
     return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_kv4_extend)>(g_entry[KV4_EXTEND])(cache, slots, counts, static_cast<int32_t>(count), shortfall,
-                                                                                              ws, bytes, c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_kv4_extend)>(g_entry[KV4_EXTEND])(cache, slots, counts, static_cast<int32_t>(count), shortfall,
+        ws, bytes, c.stream);
+  });
 }
 
 // fork(cache, src, dst, deep, shortfall, workspace, stream)
@@ -234,8 +258,10 @@ PyObject* fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!args_are(n, 7) || !begin(a[6], &c) || !cache_of(a[0], c, &cache) || !integers(a[1], "src", c, 0, &src, &count) ||
       !integers(a[2], "dst", c, count, &dst) || !whole(a[3], &deep) || !integers(a[4], "shortfall", c, 1, &shortfall) || !space(a[5], c, &ws, &bytes))
     return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_kv4_fork)>(g_entry[KV4_FORK])(cache, src, dst, static_cast<int32_t>(count), deep, shortfall, ws,
-                                                                                          bytes, c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_kv4_fork)>(g_entry[KV4_FORK])(cache, src, dst, static_cast<int32_t>(count), deep, shortfall, ws,
+        bytes, c.stream);
+  });
 }
 
 // free(cache, slots, keep, stream)
@@ -247,7 +273,9 @@ PyObject* free_(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!args_are(n, 4) || !begin(a[3], &c) || !cache_of(a[0], c, &cache) || !integers(a[1], "slots", c, 0, &slots, &count) ||
       !integers(a[2], "keep", c, count, &keep))
     return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_kv4_free)>(g_entry[KV4_FREE])(cache, slots, keep, static_cast<int32_t>(count), c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_kv4_free)>(g_entry[KV4_FREE])(cache, slots, keep, static_cast<int32_t>(count), c.stream);
+  });
 }
 
 // compact(cache, live, workspace, stream)
@@ -258,7 +286,9 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* ws;
   size_t bytes;
   if (!args_are(n, 4) || !begin(a[3], &c) || !cache_of(a[0], c, &cache) || !integers(a[1], "live", c, 1, &live) || !space(a[2], c, &ws, &bytes)) return nullptr;
-  return PyLong_FromLong(reinterpret_cast<decltype(&phobos_kv4_compact)>(g_entry[KV4_COMPACT])(cache, live, ws, bytes, c.stream));
+  return unlocked([&] {
+    return reinterpret_cast<decltype(&phobos_kv4_compact)>(g_entry[KV4_COMPACT])(cache, live, ws, bytes, c.stream);
+  });
 }
 
 // setup(entries, types, error, get_device, get_stream): addresses in the order of Entry, torch's types in the order of g_types

@@ -185,3 +185,63 @@ def test_the_short_calls_module_names_its_interpreter_and_is_left_out_without_he
     monkeypatch.setattr(serve, "LIB_PATH", tmp_path / "libphobos_leaf.so")
     with pytest.raises(ImportError, match="_bind"):
         serve.gemv_q4(None, None, None, 64)
+
+
+SLEEPER = """
+import ctypes, importlib.util, sys, threading, time
+spec = importlib.util.spec_from_file_location("_bind", sys.argv[1])
+bind = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(bind)
+
+class Ints:                                # what the module asks of an int32 tensor
+    dtype = "i32"
+    get_device = lambda self: 0
+    is_contiguous = lambda self: True
+    numel = lambda self: 4
+    data_ptr = lambda self: 4096
+    element_size = lambda self: 4
+
+usleep = ctypes.cast(ctypes.CDLL(None).usleep, ctypes.c_void_p).value
+bind.setup((usleep,) * 8, ("f16", "f32", "i8", "u8", Ints.dtype), RuntimeError, lambda: 0, lambda d: 0)
+ticks, stop = [], threading.Event()
+
+def tick():
+    while not stop.is_set():
+        ticks.append(time.monotonic())
+        time.sleep(0.001)
+
+other = threading.Thread(target=tick)
+other.start()
+cache = (500000, 0)                        # the entry point's first argument: half a second
+for call in (lambda: bind.free(cache, Ints(), None, None), lambda: bind.compact(cache, Ints(), None, None), lambda: bind.extend(cache, Ints(), Ints(), Ints(), None, None),
+             lambda: bind.fork(cache, Ints(), Ints(), 0, Ints(), None, None)):
+    t0 = time.monotonic()
+    assert call() == 0
+    t1 = time.monotonic()
+    assert t1 - t0 >= 0.4, t1 - t0
+    print(sum(t0 + 0.1 < t < t1 - 0.1 for t in list(ticks)))
+stop.set()
+other.join()
+# two threads' calls are made one after another
+t0 = time.monotonic()
+both = [threading.Thread(target=lambda: bind.free(cache, Ints(), None, None)) for _ in range(2)]
+for t in both:
+    t.start()
+for t in both:
+    t.join()
+assert time.monotonic() - t0 >= 0.9
+"""
+
+
+def test_other_threads_run_while_a_call_waits(ph):
+    """An entry point that takes its time (here: usleep in their place) does not hold the interpreter's lock: a launch may
+    wait for a host function that needs it.  Two threads' calls still do not mix their launches."""
+    import subprocess
+    import sys
+
+    import __graft_entry__ as entry
+    bind = entry._load_build_module().BIND
+    r = subprocess.run([sys.executable, "-c", SLEEPER, str(bind)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    counts = [int(x) for x in r.stdout.split()]
+    assert len(counts) == 4 and all(c > 0 for c in counts), counts
