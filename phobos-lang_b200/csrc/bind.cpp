@@ -132,6 +132,11 @@ bool space(PyObject* t, const Call& c, void** at, size_t* bytes) {
   *at = nullptr;
   *bytes = 0;
   if (t == Py_None) return true;
+  PyObject* contiguous = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+  if (!contiguous) return false;
+  Py_DECREF(contiguous);  // True and False stay
+  // (a view that repeats its elements has more of them than bytes of memory)
+  if (contiguous != Py_True) return refuse(PH_ERR_WORKSPACE, "%s: not contiguous", "workspace");
   long long address, n, each;
   if (!on_device(t, "workspace", c) || !integer(t, s_data_ptr, &address) || !integer(t, s_numel, &n) || !integer(t, s_element_size, &each)) return false;
   *at = reinterpret_cast<void*>(address);

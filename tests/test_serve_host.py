@@ -245,3 +245,47 @@ def test_other_threads_run_while_a_call_waits(ph):
     assert r.returncode == 0, r.stderr
     counts = [int(x) for x in r.stdout.split()]
     assert len(counts) == 4 and all(c > 0 for c in counts), counts
+
+
+WORKSPACES = """
+import importlib.util, sys
+spec = importlib.util.spec_from_file_location("_bind", sys.argv[1])
+bind = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(bind)
+import torch
+
+class Device:                              # a tensor in host memory that says it is on device 0
+    def __init__(self, t):
+        self.t, self.dtype = t, t.dtype
+
+    def __getattr__(self, name):
+        return (lambda: 0) if name == "get_device" else getattr(self.t, name)
+
+class Refused(Exception):
+    pass
+
+import ctypes
+called = []
+entry = ctypes.CFUNCTYPE(ctypes.c_int, *[ctypes.c_void_p] * 5)(lambda cache, live, ws, n, stream: called.append(n) or 0)
+bind.setup((ctypes.cast(entry, ctypes.c_void_p).value,) * 8, (torch.float16, torch.float32, torch.int8, torch.uint8, torch.int32), Refused, lambda: 0, lambda d: 0)
+live = Device(torch.zeros(1, dtype=torch.int32))
+space = torch.zeros(64, dtype=torch.uint8)
+assert bind.compact((4096, 0), live, Device(space), None) == 0 and called == [64]
+for view in (space[:1].expand(1 << 20), space.view(8, 8).t(), space[::2]):
+    try:
+        bind.compact((4096, 0), live, Device(view), None)
+    except Refused as e:
+        assert "workspace" in str(e)
+    else:
+        raise SystemExit(f"taken: {view.stride()}, {called}")
+"""
+
+
+def test_a_workspace_is_contiguous(ph):
+    """A view that repeats its elements has fewer bytes behind its address than elements: not a workspace."""
+    import subprocess
+    import sys
+
+    import __graft_entry__ as entry
+    r = subprocess.run([sys.executable, "-c", WORKSPACES, str(entry._load_build_module().BIND)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
