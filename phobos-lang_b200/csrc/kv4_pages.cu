@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_plan_kernel(Kv4View c, Pl
   }
   claim_rows(c, p, slots, n);
   const int in_page = (1 << c.page_shift) - 1;
+  bool shares = false;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int slot = slots[i], add = counts[i];
     int fresh = 0, last = -1;
@@ -166,27 +167,37 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_plan_kernel(Kv4View c, Pl
         fresh = pages_for(c, len + add) - have;
         if (add > 0 && (len & in_page)) {
           const int page = c.tables[static_cast<long long>(slot) * c.table_width + have - 1];
-          if (page < 0 || page >= c.n_pages)
+          if (page < 0 || page >= c.n_pages) {
             wrong = 1;
-          else if (c.refs[page] > 1)
+          } else if (c.refs[page] > 1) {
             last = page;
+            shares = true;
+            p.moves[page] = make_int2(0, -1);
+          }
         }
       }
     }
     p.fresh[i] = fresh;
     p.last[i] = last;
   }
-  __syncthreads();
-  // of the rows that extend one shared page, all but those that are left alone with it copy it: what doing them one
-  // after another would give
-  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-    const int last = p.last[i];
-    if (last < 0) continue;
-    int before = 0;
-    for (int j = 0; j < i; j++) before += p.last[j] == last;
-    if (c.refs[last] - before > 1) p.fresh[i]++;
+  // Of the rows that extend one shared page all copy it, but where they are all that hold it the last one keeps it: what doing
+  // them one after another would give.  The moves' places are free until then and count the rows of each such page.
+  if (__syncthreads_or(shares)) {
+    for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
+      if (p.last[i] >= 0) {
+        atomicAdd(&p.moves[p.last[i]].x, 1);
+        atomicMax(&p.moves[p.last[i]].y, i);
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+      const int last = p.last[i];
+      if (last < 0) continue;
+      const int2 rows = __ldcg(&p.moves[last]);
+      if (rows.x > c.refs[last]) wrong = 1;  // (more tables name the page than its count says)
+      if (rows.x < c.refs[last] || rows.y != i) p.fresh[i]++;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   // a row's fresh pages beyond those its length asks for are the copy's
   const long long want = scan_fresh(p, n);
   if (wrong) {

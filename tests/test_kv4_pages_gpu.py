@@ -272,3 +272,45 @@ def test_refusals(ph, dev):
         with pytest.raises(ph.PhobosError):
             f()
     b.same(None)
+
+
+def test_many_branches_grow_at_once(ph, dev):
+    """Thousands of rows that extend one shared page, with and without the row that keeps it, and pages shared by a few; the
+    plan's time must not grow with the square of the rows (20000 rows took 14 times what as many without a shared page take
+    with a loop over all earlier rows, now twice; the limit is six times)."""
+    import torch
+    n = 20000
+    b = Both(ph, dev, n_pages=2 * n + 300, seqs=n + 10, width=2, page=16, layers=1)
+    b.extend([0, 1, 2], [5, 21, 16])
+    b.fork([0] * (n - 100), list(range(10, n - 90)))
+    b.fork([1] * 60 + [2] * 40, list(range(n - 90, n + 10)))
+    r = random.Random(3)
+    rows = list(range(10, n - 90, 2)) + list(range(n - 90, n + 10))
+    r.shuffle(rows)
+    assert b.extend(rows, [r.choice([0, 1, 3]) for _ in rows]) == 0
+    rows = [0, 1, 2] + list(range(11, n - 90, 2))      # all that still hold the page: the last of them keeps it
+    r.shuffle(rows)
+    assert b.extend(rows, [1] * len(rows)) == 0
+
+    def best(shared):
+        c = ph.Kv4Cache.create(1, 2 * n + 8, 1, 64, 64, 16, n + 1, 2)
+        ws = torch.empty(ph.kv4_pages_workspace_bytes(c), dtype=torch.uint8, device=dev)
+        slots, one, out, times = torch.arange(n, device=dev, dtype=torch.int32), torch.ones(n, dtype=torch.int32, device=dev), b.ints([0]), []
+        for _ in range(5):
+            c.refs.zero_()
+            c.lens[:n] = 5
+            if shared:
+                c.refs[0] = n
+                c.tables[:n, 0] = 0
+            else:
+                c.refs[:n] = 1
+                c.tables[:n, 0] = slots
+            start, end = torch.cuda.Event(True), torch.cuda.Event(True)
+            start.record()
+            ph.kv4_extend(c, slots, one, out, workspace=ws)
+            end.record()
+            assert int(out) == 0
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert best(True) <= 6 * best(False)
