@@ -125,6 +125,7 @@ int map_launch_rc(int rc, const char* what, const char* err) {
   if (rc == 0) return PH_OK;
   if (rc == -2) return fail(PH_ERR_UNSUPPORTED, "%s: %s", what, err);
   if (rc == -1) return fail(PH_ERR_INVALID, "%s: %s", what, err);
+  cudaGetLastError();  // reported here; the runtime would hand it to the next caller that asks
   return fail(PH_ERR_DEVICE, "%s: %s", what, err);
 }
 

@@ -242,6 +242,7 @@ struct PackParams {
 
 // One CTA of 256 threads: one block; thread i writes one 4-byte word of codes (eight codes of two rows).
 __global__ void __launch_bounds__(256) q4_pack_kernel(PackParams p) {
+  pdl_wait();
   const int kb = blockIdx.x % p.kblocks, tile = blockIdx.x / p.kblocks, tid = threadIdx.x;
   uint8_t* blk = p.out + static_cast<long long>(blockIdx.x) * p.block_bytes;
   const int lane = (tid & 127) >> 2, w = (tid >> 7) * 4 + (tid & 3), g = lane >> 2, t = lane & 3;
@@ -268,13 +269,6 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(PackParams p) {
   }
 }
 
-int launched(const char** err) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return 0;
-  *err = cudaGetErrorString(e);
-  return -3;
-}
-
 }  // namespace
 
 size_t q4_packed_bytes(long long N, long long K, int group) {
@@ -290,8 +284,10 @@ int launch_q4_pack(const void* codes, long long ldc, const void* scales, long lo
     *err = "more than 2^31 - 1 blocks of weights";
     return -2;
   }
-  q4_pack_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-  return launched(err);
+  const cudaError_t e = launch_with_pdl(q4_pack_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+  if (e == cudaSuccess) return 0;
+  *err = cudaGetErrorString(e);
+  return -3;
 }
 
 namespace {

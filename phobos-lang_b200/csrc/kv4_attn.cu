@@ -764,7 +764,6 @@ int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace
                 : launch_rows_of<128, 4>(p, nt, most_rows, sm_count, stream);
   else
     e = ng == 1 ? launch_rows_of<64, 1>(p, nt, most_rows, sm_count, stream) : launch_rows_of<64, 2>(p, nt, most_rows, sm_count, stream);
-  if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess) return 0;
   *err = cudaGetErrorString(e);
   return -3;

@@ -145,3 +145,40 @@ def test_two_caches_on_two_streams(ph, dev):
     for a, b in zip(alone, outs):
         assert torch.equal(a, b)
     assert ph.device_status() == 0
+
+
+def test_a_launch_that_fails_is_reported_once(ph, dev):
+    """A launch that CUDA refuses (into the legacy stream while a stream that orders itself after it is being captured) is an
+    error of that call alone: the next calls neither report it nor do without their work."""
+    import torch
+    from cuda.bindings import runtime
+    L = Layer(ph, dev)
+    x = torch.randn(3, 256, device=dev).half()
+    y, again = torch.empty(3, 512, device=dev), torch.zeros(3, 512, device=dev)
+    ph.gemv_q4(x, L.packed["q"], y, L.G)
+    L.step(x, [2], [3])
+    code = torch.randint(0, 16, (512, 256), dtype=torch.uint8, device=dev)
+    scale = torch.rand(512, 4, device=dev).half()
+    packed = ph.q4_pack(code, scale, None, L.G)
+    out, slots = torch.zeros_like(packed), L.ints([2])
+    q, o, o2 = torch.randn(1, 512, device=dev).half(), torch.empty(1, 512, device=dev).half(), torch.zeros(1, 512, device=dev).half()
+    ph.kv4_attention(L.cache, 0, q, o, 0.125, slots, workspace=L.ws)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    calls = [lambda: ph.q4_pack(code, scale, None, L.G, out=out, stream=side), lambda: ph.kv4_attention(L.cache, 0, q, o2, 0.125, slots, workspace=L.ws, stream=side),
+             lambda: ph.gemv_q4(x, L.packed["q"], again, L.G, stream=side)]
+    for call in calls:
+        err, stream = runtime.cudaStreamCreate()
+        assert int(err) == 0
+        assert int(runtime.cudaStreamBeginCapture(stream, runtime.cudaStreamCaptureMode.cudaStreamCaptureModeRelaxed)[0]) == 0
+        try:
+            with pytest.raises(ph.PhobosError) as e:
+                ph.gemv_q4(x, L.packed["q"], y, L.G, stream=0)
+            assert e.value.code == ph.PH_ERR_DEVICE
+        finally:
+            runtime.cudaStreamEndCapture(stream)
+            runtime.cudaStreamDestroy(stream)
+        call()
+    torch.cuda.synchronize()
+    assert torch.equal(out, packed) and torch.equal(o, o2) and torch.equal(y, again)
+    assert ph.device_status() == 0
