@@ -416,7 +416,9 @@ TcGemvSplit tc_gemv_split(int tiles, int kblocks, int m_groups, int sm_count) {
   return s;
 }
 
-int columns_for(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+// Columns of the product.  (With four groups to a block sixteen of them never pay: 0.79 us a block and round for up to 1184
+// tiles, which the other kernel takes 0.66 for.)
+int columns_for(int M, int group) { return M <= 16 && group > 32 ? 16 : M <= 32 ? 32 : 64; }
 
 template <int NC, int GS>
 cudaError_t launch_shape(const CUtensorMap& x_map, TcGemvParams& p, int sm_count, cudaStream_t stream) {
@@ -441,15 +443,17 @@ cudaError_t launch_shape(const CUtensorMap& x_map, TcGemvParams& p, int sm_count
 
 template <int GS>
 int launch_group(const void* X, long long ldx, TcGemvParams& p, int sm_count, cudaStream_t stream, const char** err) {
-  const int nc = columns_for(p.M);
+  const int nc = columns_for(p.M, 16 * GS);
   CUtensorMap x_map;
   if (!make_tmap_2d(&x_map, X, TMAP_F16, p.M, p.K, ldx, nc, 64, TMAP_SWIZZLE_128B)) {
     *err = "cuTensorMapEncodeTiled failed (alignment or driver entry point)";
     return -1;
   }
-  const cudaError_t e = nc == 16   ? launch_shape<16, GS>(x_map, p, sm_count, stream)
-                        : nc == 32 ? launch_shape<32, GS>(x_map, p, sm_count, stream)
-                                   : launch_shape<64, GS>(x_map, p, sm_count, stream);
+  cudaError_t e = cudaSuccess;
+  if constexpr (GS > 2)
+    if (nc == 16) e = launch_shape<16, GS>(x_map, p, sm_count, stream);
+  if (nc == 32) e = launch_shape<32, GS>(x_map, p, sm_count, stream);
+  if (nc == 64) e = launch_shape<64, GS>(x_map, p, sm_count, stream);
   if (e == cudaSuccess) return 0;
   *err = cudaGetErrorString(e);
   return -3;
@@ -462,7 +466,7 @@ int launch_group(const void* X, long long ldx, TcGemvParams& p, int sm_count, cu
 // 128: 31, 35, 55 us for 16, 32, 64 rows of X); the other 3.5 us and 0.28 ns for each 16 x 128 block and eight rows of X,
 // which it reads the weights anew for (39, 76, 151 us; but 4096 x 4096: 9, 16, 30 us against 13, 17, 27).
 bool gemv_q4_tc_is_faster(int M, int N, int K, int group, int sm_count) {
-  const int nc = columns_for(M), m_groups = (M + nc - 1) / nc, tiles = (N + 15) / 16, kblocks = (K + 127) / 128;
+  const int nc = columns_for(M, group), m_groups = (M + nc - 1) / nc, tiles = (N + 15) / 16, kblocks = (K + 127) / 128;
   const TcGemvSplit s = tc_gemv_split(tiles, kblocks, m_groups, sm_count);
   const double here = 4.0 + (s.split > 1 ? 4.0 : 0.0) + static_cast<double>(s.rounds) * ((kblocks + s.split - 1) / s.split) *
                                                            (0.25 + 128 / group * (0.03 + 0.0065 * nc));
