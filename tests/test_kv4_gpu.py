@@ -514,3 +514,33 @@ def test_values_over_the_whole_range_give_finite_outputs(ph, dev, length):
     ph.kv4_append(s.cache, 0, s.k, s.v, s.slots, ind)
     o, _ = attend(s, torch.randn(1, 2 * D, device=dev).half(), [0, 1], 0.125)
     assert bool(torch.isnan(o.view(2, D)[:, :G]).all()) and bool(torch.isfinite(o.view(2, D)[:, G:]).all())
+
+
+@pytest.mark.parametrize("D,G,rep,page", [(128, 128, 4, 64), (128, 32, 16, 128), (64, 64, 1, 16)])
+def test_alone_and_in_a_batch(ph, dev, D, G, rep, page):
+    """A sequence attended alone and in batches whose other sequences move the places where it is cut: each within the
+    tolerance of the definition, and so within the sum of both of one another.  A window and several rows a sequence too."""
+    import torch
+    lens, new = [3000, 17, 1200, 64, 9000, 1], [1, 3, 1, 2, 1, 1]
+    s = Setup(ph, dev, lens, 2, D, G, page, seed=21)
+    ind = [0, *np.cumsum(new).tolist()]
+    q = torch.randn(ind[-1], 2 * rep * D, device=dev).half()
+    scale = 1 / math.sqrt(D)
+    for window in (0, 700):
+        wo, wl, to, tl = reference(s, q, ind, rep, scale, window)
+        near = lambda got, want, tol: bool(((got.double() - want).abs() <= tol).all())  # noqa: E731
+        o, lse = attend(s, q, ind, scale, window)
+        assert near(o, wo, to) and near(lse, wl, tl)
+        for b in range(len(lens)):
+            a, z = ind[b], ind[b + 1]
+            o1, lse1 = attend(s, q[a:z].contiguous(), [0, z - a], scale, window, slots=s.slots[b:b + 1])
+            assert near(o1, wo[a:z], to[a:z]) and near(lse1, wl[a:z], tl[a:z])
+            assert near(o1, o[a:z].double(), 2 * to[a:z]) and near(lse1, lse[a:z].double(), 2 * tl[a:z])
+        half = [4, 1, 0]
+        i = [0]
+        for b in half:
+            i.append(i[-1] + new[b])
+        rows = torch.cat([torch.arange(ind[b], ind[b + 1]) for b in half]).to(dev)
+        o2, lse2 = attend(s, q[rows].contiguous(), i, scale, window, slots=s.slots[torch.tensor(half, device=dev)].contiguous())
+        assert near(o2, wo[rows], to[rows]) and near(lse2, wl[rows], tl[rows])
+    assert ph.device_status() == 0

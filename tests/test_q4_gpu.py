@@ -296,3 +296,42 @@ def test_the_switch_for_early_starts_reaches_every_form(ph, dev, pdl):
     assert r.returncode == 0, r.stderr[-2000:]
     word, edges, early = r.stdout.split()
     assert (word, edges) == ("edges", "5") and (int(early) > 0) == (pdl == "1")
+
+
+# forms that the sizes above leave out: sixteen columns with G = 64, 32 columns with G = 32, 64 columns with G = 64, and shares
+# along K for clusters of two and of four, with even, odd and unequal shares
+MORE = [(9, 18766, 448, 64), (16, 18930, 2112, 64), (31, 56074, 160, 32), (32, 18930, 2080, 32), (48, 16390, 1152, 64), (64, 14133, 4096, 64),
+        (64, 2048, 8192, 128), (58, 2220, 4736, 128), (29, 2327, 15232, 128), (128, 1125, 22272, 64), (29, 4608, 7680, 128), (61, 4619, 12160, 64),
+        (2048, 51, 5120, 128)]
+
+
+@pytest.mark.parametrize("M,N,K,G", MORE)
+def test_tensor_core_forms_left(ph, dev, M, N, K, G):
+    import torch
+    g = torch.Generator().manual_seed(M + K)
+    x = (torch.randn(M, K, generator=g) + 0.5).half().to(dev)
+    code, scale, zero = _weights(N, K, G, N + K, dev, zeros=M % 2 == 0)
+    w = ph.q4_pack(code, scale, zero, G)
+    y, z = torch.full((M, N), float("nan"), device=dev), torch.full((M, N), float("nan"), device=dev)
+    ph.gemv_q4(x, w, y, G)
+    want, S = _want(x, code, scale, zero, G)
+    assert bool(((y.double() - want).abs() <= _tol(S, want, K, G, False)).all())
+    ph.gemv_q4(x, w, z, G)
+    assert torch.equal(y, z) and ph.device_status() == 0
+
+
+@pytest.mark.parametrize("G,K", [(128, 1152), (64, 448), (32, 416)])
+@pytest.mark.parametrize("M,N", [(1, 5003), (7, 9401), (8, 9501), (2, 18901), (3, 20011), (1, 40007), (13, 9501)])
+def test_warp_level_forms(ph, dev, M, N, G, K):
+    """Shares of one to more than eight tiles a CTA: each shape of the warp-level kernel, with tiles and columns left over.
+    (13 rows: the 128 and 64 groups may take the tensor-core form.)"""
+    import torch
+    g = torch.Generator().manual_seed(M + N)
+    x = (torch.randn(M, K, generator=g) - 0.25).half().to(dev)
+    code, scale, zero = _weights(N, K, G, N + K, dev, zeros=M != 2)
+    w = ph.q4_pack(code, scale, zero, G)
+    buf = torch.full((M, N + 3), float("nan"), device=dev)
+    ph.gemv_q4(x, w, buf[:, 1:1 + N], G)
+    want, S = _want(x, code, scale, zero, G)
+    assert bool(((buf[:, 1:1 + N].double() - want).abs() <= _tol(S, want, K, G, False)).all())
+    assert bool(torch.isnan(buf[:, [0, N + 1, N + 2]]).all()) and ph.device_status() == 0
