@@ -544,3 +544,49 @@ def test_alone_and_in_a_batch(ph, dev, D, G, rep, page):
         o2, lse2 = attend(s, q[rows].contiguous(), i, scale, window, slots=s.slots[torch.tensor(half, device=dev)].contiguous())
         assert near(o2, wo[rows], to[rows]) and near(lse2, wl[rows], tl[rows])
     assert ph.device_status() == 0
+
+
+def test_pages_beyond_four_gigabytes(ph, dev):
+    """Offsets that pass 32 bits: pages and a second layer behind the first 2^32 bytes are written, read, attended, copied
+    and moved like any others."""
+    import torch
+    H, D, G, page = 8, 128, 32, 256
+    n_pages, seqs = 16500, 4
+    c = ph.Kv4Cache.create(2, n_pages, H, D, G, page, seqs, 3)
+    assert c.pages[0].numel() > 2 ** 32
+    low = 16480
+    c.refs[:low] = 1                                     # the pages in front are taken
+    ws = torch.empty(max(ph.kv4_pages_workspace_bytes(c), ph.kv4_attention_workspace_bytes(c, 1, 1, 2 * H)), dtype=torch.uint8, device=dev)
+    out = torch.zeros(1, dtype=torch.int32, device=dev)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    n = 600
+    ph.kv4_extend(c, ints(2), ints(n), out, workspace=ws)
+    assert int(out) == 0 and c.tables[2].tolist() == [low, low + 1, low + 2]
+    k, v = (torch.randn(n, H * D, device=dev).half() for _ in range(2))
+    q = torch.randn(1, 2 * H * D, device=dev).half()
+
+    def right(slot, layer):
+        for rows in (k, v):
+            got = [torch.empty_like(k), torch.empty_like(v)]
+            ph.kv4_read(c, layer, *got, ints(slot), ints(0, n))
+            want = value(rows.unflatten(1, (H, D)), G).flatten(1)
+            assert bool(((got[rows is v].double() - want).abs() <= 2.0 ** -11 * want.abs() * 1.001 + 2.0 ** -23).all())
+        s = Setup.__new__(Setup)
+        s.ph, s.dev, s.Hkv, s.D, s.G, s.lens, s.ind, s.k, s.v = ph, dev, H, D, G, [n], [0, n], k, v
+        want, _, tol, _ = reference(s, q, [0, 1], 2, 0.09, 0)
+        o = torch.empty_like(q)
+        ph.kv4_attention(c, layer, q, o, 0.09, ints(slot), workspace=ws)
+        assert bool(((o.double() - want).abs() <= tol).all())
+
+    for layer in (0, 1):
+        ph.kv4_append(c, layer, k, v, ints(2), ints(0, n))
+    right(2, 0), right(2, 1)
+    ph.kv4_fork(c, ints(2), ints(0), out, deep=True, workspace=ws)
+    assert int(out) == 0 and c.tables[0].tolist() == [low + 3, low + 4, low + 5]
+    ph.kv4_free(c, ints(2))
+    right(0, 1)
+    c.refs[:low] = 0                                     # now the copies are all there is: they move to the front
+    ph.kv4_compact(c, out, workspace=ws)
+    assert int(out) == 3 and c.tables[0].tolist() == [0, 1, 2]
+    right(0, 0), right(0, 1)
+    assert ph.device_status() == 0

@@ -335,3 +335,22 @@ def test_warp_level_forms(ph, dev, M, N, G, K):
     want, S = _want(x, code, scale, zero, G)
     assert bool(((buf[:, 1:1 + N].double() - want).abs() <= _tol(S, want, K, G, False)).all())
     assert bool(torch.isnan(buf[:, [0, N + 1, N + 2]]).all()) and ph.device_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 20])
+def test_weights_beyond_four_gigabytes(ph, dev, M):
+    """Packed weights of more than 2^32 bytes: the last rows of Y against the sum in 64 bits."""
+    import torch
+    N, K, G = 65541, 131072, 128
+    code = torch.randint(0, 16, (N, K), dtype=torch.uint8, device=dev)
+    scale = (torch.rand(N, K // G, device=dev) * 0.1 + 1e-3).half()
+    zero = (torch.rand(N, K // G, device=dev) * 20 - 2).half()
+    w = ph.q4_pack(code, scale, zero, G)
+    assert w.numel() > 2 ** 32
+    x = torch.randn(M, K, device=dev).half()
+    y = torch.empty(M, N, device=dev)
+    ph.gemv_q4(x, w, y, G)
+    for a, z in ((0, 40), (32760, 32800), (N - 40, N)):
+        want, S = _want(x, code[a:z], scale[a:z], zero[a:z], G)
+        assert bool(((y[:, a:z].double() - want).abs() <= _tol(S, want, K, G, False)).all())
+    assert ph.device_status() == 0
