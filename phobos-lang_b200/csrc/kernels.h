@@ -143,9 +143,9 @@ struct Kv4AttnArgs {
   const int* ind;       // may be null: one row per sequence
   float scale;
 };
-size_t kv4_attention_workspace(const Kv4View& c, int T, int n, int q_heads, int sm_count);
-int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, size_t workspace_bytes, int sm_count,
-                         uint32_t* status, cudaStream_t stream, const char** err);
+size_t kv4_attention_workspace(const Kv4View& c, int sm_count);  // for any batch
+int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, int sm_count, uint32_t* status,
+                         cudaStream_t stream, const char** err);
 
 // kv4_pages.cu — the pages' bookkeeping and moves.
 size_t kv4_pages_workspace(const Kv4View& c);

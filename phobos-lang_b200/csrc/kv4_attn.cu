@@ -746,12 +746,12 @@ int row_tiles(const Kv4View& c, int T, int n, int q_heads, bool one_each) { retu
 
 }  // namespace
 
-size_t kv4_attention_workspace(const Kv4View& c, int T, int n, int q_heads, int sm_count) {
+size_t kv4_attention_workspace(const Kv4View& c, int sm_count) {
   return static_cast<size_t>(sm_count) * AT_MOST_PER_SM * AT_WARPS * (sizeof(Cut) + 2 * (16 * (c.D + 2)) * sizeof(float));
 }
 
-int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, size_t workspace_bytes, int sm_count,
-                         uint32_t* status, cudaStream_t stream, const char** err) {
+int launch_kv4_attention(const Kv4View& c, const Kv4AttnArgs& a, void* workspace, int sm_count, uint32_t* status,
+                         cudaStream_t stream, const char** err) {
   Cut* cuts = static_cast<Cut*>(workspace);
   AttnParams p{c, a, a.q_heads / c.heads, 0, cuts, reinterpret_cast<float*>(cuts + sm_count * AT_MOST_PER_SM * AT_WARPS), status};
   const int nt = row_tiles(c, a.T, a.n, a.q_heads, a.ind == nullptr);

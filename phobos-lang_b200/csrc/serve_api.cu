@@ -205,8 +205,7 @@ int phobos_kv4_read(const PhKv4Cache* cache, int32_t layer, const PhTensor* K, c
 size_t phobos_kv4_attention_workspace_bytes(const PhKv4Cache* cache, int64_t T, int32_t n, int32_t q_heads) {
   Kv4View c;
   if (view_of_cache(cache, &c) || T < 0 || T > 0x7fffffffLL || n < 0 || q_heads < 1 || q_heads % c.heads != 0) return 0;
-  const int sms = sm_count_or_default();
-  return kv4_attention_workspace(c, static_cast<int>(T), n, q_heads, sms);
+  return kv4_attention_workspace(c, sm_count_or_default());
 }
 
 int phobos_kv4_attention(const PhKv4Cache* cache, int32_t layer, const PhTensor* Q, const PhTensor* O, const PhTensor* lse,
@@ -233,7 +232,7 @@ int phobos_kv4_attention(const PhKv4Cache* cache, int32_t layer, const PhTensor*
   if (window >= static_cast<long long>(c.table_width) << c.page_shift) window = 0;
   if ((rc = batch_of("kv4_attention", slots, indptr, n, q.rows))) return rc;
   const long long T = indptr ? q.rows : n;
-  const size_t need = kv4_attention_workspace(c, static_cast<int>(T), n, static_cast<int>(q_heads), sm_count_or_default());
+  const size_t need = kv4_attention_workspace(c, sm_count_or_default());
   if ((rc = workspace_of("kv4_attention", workspace, workspace_bytes, need))) return rc;
   int sms;
   uint32_t* status;
@@ -242,7 +241,7 @@ int phobos_kv4_attention(const PhKv4Cache* cache, int32_t layer, const PhTensor*
   const Kv4AttnArgs a{q.base, o.base, reinterpret_cast<float*>(l.base), q.ld, o.ld, l.ld, static_cast<int>(T), n,
                       static_cast<int>(q_heads), window, slots, indptr, scale};
   const char* err = "";
-  rc = launch_kv4_attention(c, a, workspace, workspace_bytes, sms, status, static_cast<cudaStream_t>(stream), &err);
+  rc = launch_kv4_attention(c, a, workspace, sms, status, static_cast<cudaStream_t>(stream), &err);
   return map_launch_rc(rc, "kv4_attention", err);
 }
 
