@@ -202,6 +202,7 @@ PH_API int phobos_saxpy(const PhTensor *x, const PhTensor *y, const PhTensor *ou
  * (code[n,k] - zero[n,k/group]), codes 0..15, group 32, 64 or 128, K a multiple of group.
  * X is f16, Y f16 or f32 (f32 sums, rounded once); Y is not read when beta == 0.
  * An infinity in X makes of its row of Y what the formula says: an infinity, or NaN where it meets a weight of zero.
+ * A group is summed as sum x code - zero sum x: an f32 Y is off by about 7e-7 of its size, some times a plain f32 sum's error.
  * X: rows 16-byte aligned.  Y: any N, any row stride >= N.
  * phobos_q4_pack lays weights out once, in the order the kernel reads them: codes [N,K] one
  * per byte (the low four bits count), scales and zeros [N, K/group] f16 (zeros may be NULL:
@@ -262,8 +263,11 @@ PH_API int phobos_kv4_read(const PhKv4Cache *cache, int32_t layer, const PhTenso
  * (head h reads key/value head h / (q_heads / kv_heads)).  The row of position p sees tokens j <= p, and with
  * window > 0 only j > p - window.  A row that sees nothing gets zeros.  O is at most +-65504, as values read back are.
  * lse, [T, q_heads] f32 or NULL: the natural logarithm of the sum of exp(scale * q k), -inf for a row that sees nothing.
+ * Scores, maxima and sums are f32; a weight times a value's scale is rounded to f16 once, as flash_attention rounds its
+ * weights.
  * The workspace (256-byte aligned, phobos_kv4_attention_workspace_bytes; its contents need not be kept) holds what is
- * found of one sequence in several places; calls that share one must not overlap on the GPU. */
+ * found of one sequence in several places; calls that share one must not overlap on the GPU.  It is as large for one row as
+ * for any batch (0 bytes are returned for arguments that no call takes), so one of a cache's serves every call. */
 PH_API size_t phobos_kv4_attention_workspace_bytes(const PhKv4Cache *cache, int64_t T, int32_t n, int32_t q_heads);
 PH_API int phobos_kv4_attention(const PhKv4Cache *cache, int32_t layer, const PhTensor *Q, const PhTensor *O,
                                 const PhTensor *lse, float scale, int32_t window, const int32_t *slots,
@@ -272,7 +276,8 @@ PH_API int phobos_kv4_attention(const PhKv4Cache *cache, int32_t layer, const Ph
 /* Bookkeeping.  Fresh pages are the lowest free ids, handed out in the order of the rows.  `workspace` (256-byte
  * aligned, phobos_kv4_pages_workspace_bytes; contents need not be kept).  shortfall (device, one value): 0 when done;
  * > 0 when that many pages are missing, -1 when the request is wrong (a slot out of range or listed twice, a negative
- * count, more tokens than table_width pages hold, a destination that is not empty): then nothing has changed. */
+ * count, more tokens than table_width pages hold, a destination that is not empty, more rows on a shared page than refs
+ * counts): then nothing has changed. */
 PH_API size_t phobos_kv4_pages_workspace_bytes(const PhKv4Cache *cache);
 /* Makes room for counts[i] more tokens of slots[i] and adds them to its length.  A last page that others share and
  * that the new tokens would be written to is copied, in all layers, as if the rows were taken one after another. */

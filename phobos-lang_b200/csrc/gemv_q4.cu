@@ -13,11 +13,13 @@
 // of W (RT tiles of 16 each), WK along the columns (a block of 128 each).  A stage of the ring holds WR RT x WK blocks and
 // WK * 128 columns of up to eight rows of X, brought by bulk copies; X rows stand 64 bytes off a multiple of 128 apart, so
 // that a lane's 16-byte reads (the B operand of two matrix steps) meet no bank twice.  The tiles of W are dealt out evenly
-// over a grid that fills the GPU: a CTA whose share is not a multiple of WR RT leaves some products idle, which costs
-// nothing as long as the bytes are what is waited for.
-// Measured: 1 x 28672 x 8192, G = 128: 28.2 us, 4.4 TB/s (23.4 us without the products: bound by instructions, 123 for a
-// block of 16 x 128, half of them masks and shifts); 1 x 4096 x 4096: 4.8 us back to back in a graph.  Four tiles a warp
-// (x read and summed once for all of them) took 31 us where two took 34, sixteen rows a CTA in every case 37.
+// over a grid that fills the GPU.  A CTA whose share is not a multiple of WR RT does the products of the places without a
+// tile all the same, on what the ring held; that is part of what 5 x 11001 x 4096, G = 64, pays: its CTAs have two or three
+// tiles in a shape of four, and it takes 10.9 us, 7.9 with the products left out, where the bytes are 3.9.
+// Measured: 1 x 28672 x 8192, G = 128: 27.9 us, 4.5 TB/s (23.4 us without the products; 122 instructions for a block of 16 x
+// 128, half of them masks and shifts; neither HBM nor a pipe nor the issue slots are full: half of them, by four warps a
+// scheduler that wait for loads and for the pipes in turn); 1 x 4096 x 4096: 4.9 us back to back in a graph.  Four tiles a
+// warp (x read and summed once for all of them) took 31 us where two took 34, sixteen rows a CTA in every case 37.
 #include <atomic>
 #include <type_traits>
 

@@ -22,7 +22,12 @@
 // shared memory with bulk copies (one per unit, 2176 bytes at D = G = 128) that it issues itself.
 // Measured: 64 sequences of 1..8192 tokens, 8 heads of 128, 291 MB: 62 us, 4.7 TB/s, bound by instructions (257 a unit, issued
 // in half of all slots by 12 warps to an SM).  Eight rows a problem where no more can be there, else sixteen: the widening of
-// the codes is then done once for both halves (64 query heads on 4, G = 32: 73 us against 90).
+// the codes is then done once for both halves (64 query heads on 4, G = 32: 73 us against 90).  What holds these forms back
+// is registers: at D = 128 and four groups 168 for eight rows (324 bytes of spills stored a thread, 448 loaded) and 255 for
+// sixteen (208 and 196, eight warps to an SM); two groups at sixteen rows 255 (172 and 120); D = 64 up to 160 and 100.
+// Every warp walks the batch 32 sequences at a time to find its piece, twice where there are more than 32: 256 and 1024
+// sequences of 100 to 2000 tokens (8 heads of 128) take 87 and 290 us where the bytes take 44 and 177, 4096 of 25 to 500 tokens
+// 634 against 180.
 #include <atomic>
 
 #include "kv4.cuh"

@@ -4,7 +4,9 @@
 // them, and a fresh page is always the lowest free one: the outcome does not depend on timing.  A change that needs
 // pages is planned by one CTA (counts, prefix sums, the free pages in order) and is all or nothing; the pages' bytes
 // are then moved by the whole GPU from the list that the plan left in the workspace.
-// Measured: copying 16 sequences of 2000 tokens in 16 layers, 1 GB read and written: 165 us, 6.2 TB/s; a plan 7 to 9 us.
+// Measured: copying 16 sequences of 2000 tokens in 16 layers, 1 GB read and written: 165 us, 6.2 TB/s.  A plan
+// takes 7 to 9 us for up to 48 rows and grows with them: extending 1000, 4096 and 65536 branches of one prompt takes 46, 126
+// and 2281 us in all, as many sequences that share nothing 29, 69 and 1113.
 #include "kv4.cuh"
 
 namespace ph {
