@@ -217,7 +217,8 @@ PH_API int phobos_gemv_q4(const PhTensor *X, const PhTensor *packed, const PhTen
 /* ---- key/value cache in 4 bits ------------------------------------------------------- *
  * No counterpart in the reference: flash_attention's keys and values kept between calls, in
  * pages, as 4-bit codes with an f16 (scale, zero) pair per group of dims:
- *   scale = f16((max - min) / 15), zero = min, code = rint((x - min) / scale)
+ *   scale = f16((max - min) / 15), zero = min, code = rint((x - min) / scale), 15 at most
+ *   (the differences in f32: beside a large min the last bits of the smallest x do not count)
  *   value = zero + scale * code
  * A group that holds a value that is not finite reads back as NaN.  All arrays are device
  * memory of the caller:

@@ -524,7 +524,7 @@ def test_alone_and_in_a_batch(ph, dev, D, G, rep, page):
     lens, new = [3000, 17, 1200, 64, 9000, 1], [1, 3, 1, 2, 1, 1]
     s = Setup(ph, dev, lens, 2, D, G, page, seed=21)
     ind = [0, *np.cumsum(new).tolist()]
-    q = torch.randn(ind[-1], 2 * rep * D, device=dev).half()
+    q = torch.randn(ind[-1], 2 * rep * D, generator=torch.Generator().manual_seed(22)).half().to(dev)
     scale = 1 / math.sqrt(D)
     for window in (0, 700):
         wo, wl, to, tl = reference(s, q, ind, rep, scale, window)
@@ -559,11 +559,10 @@ def test_pages_beyond_four_gigabytes(ph, dev):
     ws = torch.empty(max(ph.kv4_pages_workspace_bytes(c), ph.kv4_attention_workspace_bytes(c, 1, 1, 2 * H)), dtype=torch.uint8, device=dev)
     out = torch.zeros(1, dtype=torch.int32, device=dev)
     ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
-    n = 600
+    n, g = 600, torch.Generator().manual_seed(41)
     ph.kv4_extend(c, ints(2), ints(n), out, workspace=ws)
     assert int(out) == 0 and c.tables[2].tolist() == [low, low + 1, low + 2]
-    k, v = (torch.randn(n, H * D, device=dev).half() for _ in range(2))
-    q = torch.randn(1, 2 * H * D, device=dev).half()
+    k, v, q = (torch.randn(rows, heads * D, generator=g).half().to(dev) for rows, heads in ((n, H), (n, H), (1, 2 * H)))
 
     def right(slot, layer):
         for rows in (k, v):
