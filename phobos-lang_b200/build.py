@@ -17,7 +17,7 @@ CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 LIB = HERE / "libphobos_leaf.so"
 # CPython module of serve.py's short calls; the suffix names the interpreter it was built for
-BIND = HERE / ("_bind" + sysconfig.get_config_var("EXT_SUFFIX") or ".so")
+BIND = HERE / ("_bind" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_f32.cu", "flash.cu", "elementwise.cu", "kda.cu", "tmap.cu", "noalloc.cu", "selftest.cu",
            "gemv_q4.cu", "gemv_q4_tc.cu", "kv4_cache.cu", "kv4_attn.cu", "kv4_pages.cu", "serve_api.cu",
            "host.cpp", "executor.cpp", "source.cpp", "planner.cpp", "plan_api.cpp", "wire.cpp"]

@@ -33,7 +33,7 @@ _bind = None           # the CPython module with the short calls (csrc/bind.cpp)
 def _load():
     """Loads csrc/bind.cpp's module and gives it what it calls; raises if it has not been built (no fallback exists)."""
     global _bind
-    path = LIB_PATH.parent / ("_bind" + sysconfig.get_config_var("EXT_SUFFIX") or ".so")
+    path = LIB_PATH.parent / ("_bind" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
     if not path.exists():
         raise ImportError(f"{path} is missing: build it with `python phobos-lang_b200/build.py`")
     import torch
